@@ -20,6 +20,11 @@ from .api import (
     supports_fused_post_expert_rmsnorm,
 )
 from .formats import BlockScaledFormat
+
+# This library's own additions, beside the reference's names that __all__ lists: what stands around the routed experts of a layer
+from ._norm import QuantizedRows, add_rms_norm
+from ._selection import select_experts
+from .api import routed_experts_few_tokens
 from . import _ops as _ops
 
 # torch.ops.dist_moe.* (operator schemas and fake implementations for tracing); no device work happens here

@@ -44,6 +44,7 @@ from . import _native as nat
 from ._call import (BWD, FWD, FWD_ALL, CallState, arguments, launch, layout_of, observed, on_device, routes_in_one_piece,
                     span)
 from ._execution import ExecutionOptions, PreparedWeight, RMSNormPostprocess
+from ._norm import QuantizedRows
 from .formats import BlockScaledFormat, format_constants
 
 
@@ -341,7 +342,8 @@ def run_block_scaled(x, ids, scores, w13_weight, w2_weight, context: Any, option
         src2 = w2_weight.source if prepared else w2_weight
         return _Mxfp8Function.apply(x, ids, scores, src13, src2, state, options,
                                     w13_weight if prepared else None, w2_weight if prepared else None)
-    x, scores = x.detach(), scores.detach()
+    rows = x.packed if isinstance(x, QuantizedRows) else None  # quantised already
+    x, scores = x.detach() if rows is None else rows, scores.detach()
     T = x.shape[0]
     p13, p2 = _weights_for_call(w13_weight, w2_weight, state, cfg)
     lay, buf = _workspace(state)
@@ -354,9 +356,14 @@ def run_block_scaled(x, ids, scores, w13_weight, w2_weight, context: Any, option
     stride = packed_row_stride(fmt, D)
     dispatch = state.dispatch.local().data_ptr()
     # ---- publish: quantise straight into the packed symmetric dispatch rows ----------------
-    nat.check(nat.lib.dm_publish_quantised(f, x.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), dispatch, stride,
-                                           xq, xs, state.routing.local().data_ptr(), T, D, K, E,
-                                           int(options.validate_expert_ids), status, st), "dm_publish_quantised")
+    if rows is not None:  # the packed rows as they are
+        nat.check(nat.lib.dm_publish(rows.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), dispatch,
+                                     state.routing.local().data_ptr(), T, stride // 2, K, E, int(options.validate_expert_ids),
+                                     status, st), "dm_publish")
+    else:
+        nat.check(nat.lib.dm_publish_quantised(f, x.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), dispatch, stride,
+                                               xq, xs, state.routing.local().data_ptr(), T, D, K, E,
+                                               int(options.validate_expert_ids), status, st), "dm_publish_quantised")
     state.barrier(state.dispatch)
     # ---- routing (rows of every expert padded to 128) -----------------------------------------
     size = (ep * T * min(K, el) + el * 127 + 127) // 128 * 128

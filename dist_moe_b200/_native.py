@@ -236,6 +236,26 @@ _SIGNATURES = {
     "dm_bf16_backward": (c_int, [_P, _P, ctypes.c_uint32, _P, _P]),
     "dm_mxfp8_forward": (c_int, [_P, _P, ctypes.c_uint32, _P, _P]),
     "dm_mxfp8_backward": (c_int, [_P, _P, ctypes.c_uint32, _P, _P]),
+    "dm_add_rmsnorm_fwd": (
+        c_int,
+        [_P, c_int64, _P, c_int, c_int64, _P, c_int, c_float, c_float, c_int64, c_int64, _P, _P, _P, _P, c_int64, _P],
+    ),
+    "dm_add_rmsnorm_shares": (c_int64, [c_int64, c_int64]),
+    "dm_add_rmsnorm_bwd": (
+        c_int, [_P, _P, _P, c_int, c_int64, _P, c_int, c_float, _P, c_int64, c_int64, _P, _P, _P, _P, _P]),
+    "dm_dequant_mxfp8_rows": (c_int, [_P, c_int64, c_int64, c_int64, _P, _P]),
+    "dm_select_experts": (
+        c_int,
+        [_P, c_int, c_int64, c_int64, c_int, c_int, c_int, _P, c_int, c_int, c_int, c_int, c_float, _P, _P, c_int, _P, c_int, _P],
+    ),
+    "dm_select_experts_bwd": (
+        c_int, [_P, c_int, c_int64, c_int64, c_int, c_int, c_int, c_int, c_float, _P, c_int, _P, c_int, _P, _P]),
+    "dm_few_tokens_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "dm_few_tokens": (
+        c_int,
+        [_P, _P, c_int, _P, c_int, _P, _P, _P, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_float, c_float, _P, c_int64,
+         c_int, _P, _P],
+    ),
     "dm_gemm_wgrad": (c_int, [Operand, Operand, _P, c_int, c_int, _P, c_int, c_int64, c_int64, c_int64, c_int, _P, _P]),
 }
 

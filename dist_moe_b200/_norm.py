@@ -1,0 +1,194 @@
+"""The residual's addition and the RMS norm in front of a layer, with MXFP8 rows for block-scaled experts.
+
+Host side of ``dm_add_rmsnorm_fwd`` / ``_bwd`` (csrc/add_rmsnorm.cu).  The quantised rows are the packed rows that an MXFP8
+inference call publishes, so that ``routed_experts`` takes them in place of bf16 tokens and copies instead of quantising.
+"""
+
+from __future__ import annotations
+
+import dataclasses
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as nat
+from ._call import on_device
+
+_TYPES = (torch.bfloat16, torch.float32)
+
+
+@dataclasses.dataclass(frozen=True, eq=False)
+class QuantizedRows:
+    """Tokens in MXFP8: ``packed`` uint8 ``[T, stride]``, a row being ``hidden_dim`` bytes E4M3, ``hidden_dim / 32`` scales
+    E8M0 and padding to 16 bytes."""
+
+    packed: torch.Tensor
+    hidden_dim: int
+
+    def __post_init__(self) -> None:
+        t, D = self.packed, self.hidden_dim
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.device.type != "cuda":
+            raise TypeError("packed must be a CUDA uint8 tensor")
+        if isinstance(D, bool) or not isinstance(D, int) or D <= 0 or D % 32:
+            raise ValueError("hidden_dim must be a positive multiple of 32")
+        if t.ndim != 2 or t.shape[1] != _row_bytes(D) or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"packed must be a contiguous, 16-byte aligned tensor of shape [T, {_row_bytes(D)}]")
+
+    @property
+    def data(self) -> torch.Tensor:
+        """The E4M3 values ``[T, hidden_dim]``, a view."""
+        return self.packed[:, :self.hidden_dim].view(torch.float8_e4m3fn)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """The scales' exponent bytes ``[T, hidden_dim / 32]``, a view: a block's values times ``2 ** (byte - 127)``."""
+        return self.packed[:, self.hidden_dim:self.hidden_dim + self.hidden_dim // 32]
+
+    def dequantize(self) -> torch.Tensor:
+        """The rows' values as bf16 ``[T, hidden_dim]`` (exact)."""
+        T, stride = self.packed.shape
+        with on_device(self.packed.device):
+            out = torch.empty(T, self.hidden_dim, dtype=torch.bfloat16, device=self.packed.device)
+            nat.check(nat.lib.dm_dequant_mxfp8_rows(self.packed.data_ptr(), stride, T, self.hidden_dim, out.data_ptr(),
+                                                    nat.stream_ptr()), "dm_dequant_mxfp8_rows", int(T > 0))
+        return out
+
+
+def _row_bytes(dim: int) -> int:
+    return (dim + dim // 32 + 15) // 16 * 16
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with its rows' elements next to one another; rows may lie apart."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _forward(x, residual, weight, eps, center, want_rstd, quantize):
+    T, D = x.shape
+    device = x.device
+    x = _rows(x)
+    y = torch.empty((T, D), dtype=torch.bfloat16, device=device)
+    total = residual_ptr = total_ptr = None
+    residual_stride = residual_f32 = 0
+    if residual is not None:
+        residual = _rows(residual)
+        total = torch.empty((T, D), dtype=residual.dtype, device=device)
+        residual_ptr, total_ptr, residual_stride = residual.data_ptr(), total.data_ptr(), residual.stride(0)
+        residual_f32 = residual.dtype is torch.float32
+    rstd = torch.empty(T, dtype=torch.float32, device=device) if want_rstd else None
+    rows, stride = None, 0
+    if quantize:
+        stride = _row_bytes(D)
+        rows = (torch.zeros if stride != D + D // 32 else torch.empty)((T, stride), dtype=torch.uint8, device=device)
+    weight = weight.contiguous()
+    nat.check(nat.lib.dm_add_rmsnorm_fwd(
+        x.data_ptr(), x.stride(0), residual_ptr, residual_f32, residual_stride, weight.data_ptr(), weight.dtype is torch.float32,
+        center, eps, T, D, total_ptr, y.data_ptr(), nat.ptr(rstd), nat.ptr(rows), stride, nat.stream_ptr()),
+        "dm_add_rmsnorm_fwd", int(T > 0))
+    return x, y, total, rstd, rows
+
+
+class _AddRmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, center):
+        with on_device(x.device):
+            kept, y, total, rstd, _ = _forward(x, residual, weight, eps, center, True, False)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(kept if residual is None else total, weight, rstd)
+        ctx.center = center
+        return y if residual is None else (y, total)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y, grad_sum=None):
+        want_x, want_residual, want_weight = ctx.needs_input_grad[:3]
+        total, weight, rstd = ctx.saved_tensors
+        if grad_y is None:  # the stream alone is differentiated
+            if grad_sum is None:
+                return None, None, None, None, None
+            return (grad_sum.to(torch.bfloat16) if want_x else None, grad_sum if want_residual else None,
+                    torch.zeros_like(weight) if want_weight else None, None, None)
+        T, D = grad_y.shape
+        device = grad_y.device
+        apart = total.dtype is torch.float32
+        with on_device(device):
+            grad_y = grad_y.contiguous()
+            if grad_sum is not None:
+                grad_sum = grad_sum.contiguous()
+            gx = torch.empty((T, D), dtype=torch.bfloat16, device=device) if want_x or (want_residual and not apart) else None
+            gr = torch.empty((T, D), dtype=torch.float32, device=device) if want_residual and apart else None
+            gw = partial = None
+            if want_weight:
+                gw = torch.empty(D, dtype=weight.dtype, device=device)
+                partial = torch.empty((nat.lib.dm_add_rmsnorm_shares(T, D), D), dtype=torch.float32, device=device)
+            if T == 0:
+                gw = gw.zero_() if want_weight else None
+            else:
+                plain = weight.contiguous()
+                nat.check(nat.lib.dm_add_rmsnorm_bwd(
+                    grad_y.data_ptr(), nat.ptr(grad_sum), total.data_ptr(), apart, total.stride(0), plain.data_ptr(),
+                    plain.dtype is torch.float32, ctx.center, rstd.data_ptr(), T, D, nat.ptr(gx), nat.ptr(gr), nat.ptr(partial),
+                    nat.ptr(gw), nat.stream_ptr()), "dm_add_rmsnorm_bwd", 2 if want_weight else 1)
+        return gx if want_x else None, (gr if apart else gx) if want_residual else None, gw, None, None
+
+
+def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: torch.Tensor | None = None, eps: float = 1e-6,
+                 gain_center: float = 0.0, quantize: bool = False):
+    """Add ``x_TD`` to the residual stream and normalise the sum for the next layer.
+
+    ``sum = x + residual`` rounded to the residual's type (bf16 or float32; without a residual ``sum`` is ``x_TD`` itself) and
+    ``y = bf16(sum / sqrt(mean(sum ** 2) + eps) * (weight + gain_center))``: the stored sum is what is normalised.  Returns
+    ``(y_TD, sum_TD)``, differentiable in ``x_TD``, ``residual_TD`` and ``weight_D`` (bf16 or float32).  Rows may lie apart (a slice
+    of a wider tensor); other layouts are copied.
+
+    With ``quantize=True`` returns ``(y_TD, sum_TD, rows)``: ``rows`` are the MXFP8 :class:`QuantizedRows` of ``y_TD``, which
+    :func:`routed_experts` takes on MXFP8 contexts in forward-only calls, with the result that ``y_TD`` gives.  They have no
+    gradient: where one would be recorded the call raises.  ``hidden_dim`` must be a multiple of 32, at most 16384.
+    """
+    if not isinstance(x_TD, torch.Tensor) or x_TD.dtype != torch.bfloat16:
+        raise TypeError("x_TD must be a torch.bfloat16 tensor")
+    if not isinstance(weight_D, torch.Tensor) or weight_D.dtype not in _TYPES:
+        raise TypeError("weight_D must be a torch.bfloat16 or torch.float32 tensor")
+    if residual_TD is not None and (not isinstance(residual_TD, torch.Tensor) or residual_TD.dtype not in _TYPES):
+        raise TypeError("residual_TD must be a torch.bfloat16 or torch.float32 tensor")
+    if x_TD.ndim != 2 or x_TD.shape[1] == 0:
+        raise ValueError("x_TD must have shape [T, D] with D > 0")
+    D = x_TD.shape[1]
+    if weight_D.shape != (D,):
+        raise ValueError(f"weight_D must have shape [{D}]")
+    if residual_TD is not None and residual_TD.shape != x_TD.shape:
+        raise ValueError(f"residual_TD must have the shape of x_TD, {tuple(x_TD.shape)}")
+    device = x_TD.device
+    if device.type != "cuda" or weight_D.device != device or (residual_TD is not None and residual_TD.device != device):
+        raise ValueError("all operation tensors must reside on the same CUDA device")
+    if not isinstance(eps, (int, float)) or not math.isfinite(eps) or eps <= 0:
+        raise ValueError("eps must be finite and positive")
+    if not isinstance(gain_center, (int, float)) or not math.isfinite(gain_center):
+        raise ValueError("gain_center must be finite")
+    if not isinstance(quantize, bool):
+        raise TypeError("quantize must be a bool")
+    grads = torch.is_grad_enabled() and (x_TD.requires_grad or weight_D.requires_grad
+                                         or (residual_TD is not None and residual_TD.requires_grad))
+    if quantize:
+        if D % 32 or D > 16384:
+            raise ValueError("quantised rows need D to be a multiple of 32 and at most 16384")
+        if grads:
+            raise RuntimeError("quantised rows have no gradient: call add_rms_norm(quantize=True) under torch.no_grad()")
+    if grads:
+        got = _AddRmsNorm.apply(x_TD, residual_TD, weight_D, float(eps), float(gain_center))
+        return got if residual_TD is not None else (got, x_TD)
+    with on_device(device):
+        if quantize:  # the quantiser's 16-byte pieces
+            x_TD, weight_D = _aligned(x_TD), _aligned(weight_D)
+            residual_TD = None if residual_TD is None else _aligned(residual_TD)
+        _, y, total, _, rows = _forward(x_TD, residual_TD, weight_D, eps, gain_center, False, quantize)
+    if residual_TD is None:
+        total = x_TD
+    return (y, total, QuantizedRows(rows, D)) if quantize else (y, total)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    if t.data_ptr() % 16 or (t.ndim == 2 and t.stride(0) * t.element_size() % 16):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t

@@ -21,6 +21,7 @@ from typing import Any
 
 import torch
 
+from . import _few_tokens
 from . import _native as nat
 from .formats import BlockScaledFormat, format_constants
 
@@ -135,6 +136,7 @@ class ContextState:
             self.route_workspace_words = words
             self.gather_flags = torch.zeros(self.capacity_rows // 128 + 8 + ep_size * self.e_local * T // 128,
                                             dtype=torch.int32, device=device)
+            self.few_workspace = _few_tokens.workspace(self)
             self.reset()
         if config.block_scaled is not None:
             ob, vpe, sb, vec, gs = format_constants(config.block_scaled.format)
@@ -234,6 +236,7 @@ class ContextState:
     def close(self) -> None:
         torch.cuda.synchronize(self.device)
         self._native_layer = None
+        self.few_workspace = None
         self._bs_workspace = None  # a view of the arena's scratch region (block-scaled forward-only calls)
         if getattr(self, "vmm_arena", None) is not None:
             self.arena = None

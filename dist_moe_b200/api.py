@@ -21,6 +21,7 @@ import torch.distributed as dist
 
 from . import _planning
 from ._execution import DEFAULT_OPTIONS, ExecutionOptions, PreparedWeight, RMSNormPostprocess
+from ._norm import QuantizedRows
 from .formats import (
     NVFP4_DIM_MULTIPLE,
     NVFP4_HIDDEN_DIM_MAX,
@@ -573,7 +574,12 @@ def _reshape_weights(w13: torch.Tensor, w2: torch.Tensor, e_local: int, config: 
 
 
 def _validate_inputs(x, ids, scores, w13, w2, context: Context, *, prepared: bool) -> None:
-    if x.dtype != torch.bfloat16:
+    width = context.hidden_dim
+    if isinstance(x, QuantizedRows):
+        if x.hidden_dim != width:
+            raise ValueError(f"x_TD must have hidden dimension {width}")
+        x, width = x.packed, x.packed.shape[1]
+    elif x.dtype != torch.bfloat16:
         raise TypeError("x_TD must use torch.bfloat16")
     if not prepared and (w13.dtype != torch.bfloat16 or w2.dtype != torch.bfloat16):
         raise TypeError("w13_EFD and w2_EDF compute weights must use torch.bfloat16")
@@ -581,7 +587,7 @@ def _validate_inputs(x, ids, scores, w13, w2, context: Context, *, prepared: boo
         raise TypeError("topk_expert_ids_TK must use torch.int32 or torch.int64")
     if scores.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError("topk_scores_TK must use torch.bfloat16 or torch.float32")
-    if x.ndim != 2 or x.shape[1] != context.hidden_dim:
+    if x.ndim != 2 or x.shape[1] != width:
         raise ValueError(f"x_TD must have shape [T, {context.hidden_dim}]")
     T = x.shape[0]
     if not 1 <= T <= context.max_num_local_input_tokens:
@@ -599,13 +605,16 @@ def _validate_inputs(x, ids, scores, w13, w2, context: Context, *, prepared: boo
             raise ValueError("all operation tensors must be contiguous")
 
 
-def routed_experts(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tensor, topk_scores_TK: torch.Tensor,
+def routed_experts(x_TD: torch.Tensor | QuantizedRows, topk_expert_ids_TK: torch.Tensor, topk_scores_TK: torch.Tensor,
                    w13_weight: torch.Tensor | PreparedWeight, w2_weight: torch.Tensor | PreparedWeight,
                    context: Context, *, options: ExecutionOptions | None = None) -> torch.Tensor:
     """Apply the routed experts ``W2 . SwiGLU(W13 . x)`` to the local tokens.
 
     Collective over ``context.group``: every rank calls in the same order with the same
     ``T``.  Returns a fresh bf16 ``[T, D]`` tensor.  See dist_moe/api.py:3856-4112.
+
+    Forward-only calls on MXFP8 contexts also take the :class:`QuantizedRows` of ``add_rms_norm(quantize=True)`` as tokens;
+    the result is that of the bf16 tokens they were quantised from.
     """
     if not isinstance(context, Context):
         raise TypeError("context must come from create_context()")
@@ -630,14 +639,21 @@ def routed_experts(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tensor, topk_sc
     else:
         w13_EFD, w2_EDF = _reshape_weights(src13, src2, state.e_local, context.config)
         _validate_inputs(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, context, prepared=prepared)
-    if x_TD.device != state.device:
-        raise ValueError(f"x_TD is on {x_TD.device} but the context was created on {state.device}")
+    tokens = x_TD.packed if isinstance(x_TD, QuantizedRows) else x_TD
+    if tokens.device != state.device:
+        raise ValueError(f"x_TD is on {tokens.device} but the context was created on {state.device}")
     post = options.experts_output_postprocess
     norm_weight = post.weight if isinstance(post, RMSNormPostprocess) else None
-    grads = [t for t in (x_TD, topk_scores_TK, w13_EFD, w2_EDF, norm_weight) if t is not None and t.requires_grad]
+    grads = [t for t in (tokens, topk_scores_TK, w13_EFD, w2_EDF, norm_weight) if t is not None and t.requires_grad]
     if context.config.inference and grads:
         raise RuntimeError("inference contexts do not support autograd")
     save_for_backward = torch.is_grad_enabled() and bool(grads)
+    if tokens is not x_TD:
+        policy = context.config.block_scaled
+        if policy is None or policy.format is not BlockScaledFormat.MXFP8_E4M3:
+            raise ValueError("quantised tokens require an MXFP8 context")
+        if save_for_backward or options.requires_eager:
+            raise RuntimeError("quantised tokens are for forward-only calls without callbacks")
     from ._call import on_device
 
     # every launch below goes to the context's device and to that device's current stream
@@ -653,6 +669,48 @@ def routed_experts(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tensor, topk_sc
 
         return run_bf16(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_weight, w2_weight, w13_EFD, w2_EDF, context,
                         options, save_for_backward=save_for_backward)
+
+
+def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tensor, topk_scores_TK: torch.Tensor,
+                              w13_weight: torch.Tensor, w2_weight: torch.Tensor, context: Context) -> torch.Tensor:
+    """:func:`routed_experts` for a decode step of up to 64 tokens, in two launches that stream the weights of the experts hit.
+
+    ``out[t] = sum_e c[t, e] * W2[e] . SwiGLU(W13[e] . x[t])`` with ``c[t, e]`` the sum of token ``t``'s scores for expert ``e``.
+    For BF16 contexts of one rank (all experts local), forward only: a call that autograd would record raises, as do block-scaled
+    contexts and larger groups.  Products and sums are in 32 bits and the activation is rounded to bf16 once, so the result differs
+    from ``routed_experts`` in rounding.  Calls on one context are ordered, graph replays included: they share its workspace.
+    """
+    if not isinstance(context, Context):
+        raise TypeError("context must come from create_context()")
+    if context._closed:
+        raise RuntimeError("distributed MoE context is closed")
+    if isinstance(w13_weight, PreparedWeight) or isinstance(w2_weight, PreparedWeight) or context.config.block_scaled is not None:
+        raise ValueError("routed_experts_few_tokens runs on BF16 contexts with tensor weights")
+    from . import _few_tokens
+    from ._call import on_device
+
+    state = context._state
+    if state.ep != 1:
+        raise ValueError("routed_experts_few_tokens needs all experts on one rank")
+    w13_EFD, w2_EDF = _reshape_weights(w13_weight, w2_weight, state.e_local, context.config)
+    if isinstance(x_TD, QuantizedRows):
+        raise TypeError("x_TD must use torch.bfloat16")
+    _validate_inputs(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, context, prepared=False)
+    if x_TD.device != state.device:
+        raise ValueError(f"x_TD is on {x_TD.device} but the context was created on {state.device}")
+    if x_TD.shape[0] > _few_tokens.MAX_TOKENS:
+        raise ValueError(f"routed_experts_few_tokens takes at most {_few_tokens.MAX_TOKENS} tokens, got {x_TD.shape[0]}")
+    if state.few_workspace is None:
+        raise ValueError("routed_experts_few_tokens needs an intermediate dimension of whole multiples of 8, at most 1024 experts and "
+                         "a top_k of at most 32")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x_TD, topk_scores_TK, w13_EFD, w2_EDF)):
+        raise RuntimeError("routed_experts_few_tokens is forward-only: call it under torch.no_grad() or use routed_experts")
+    if x_TD.data_ptr() % 16:
+        x_TD = x_TD.clone()
+    if w13_EFD.data_ptr() % 16 or w2_EDF.data_ptr() % 16:
+        raise ValueError("w13_EFD and w2_EDF must start on a 16-byte boundary")
+    with on_device(state.device):
+        return _few_tokens.run(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, state)
 
 
 def prepare_block_scaled_weight(weight: torch.Tensor, config: Config, *, fuse_swiglu: bool = False,

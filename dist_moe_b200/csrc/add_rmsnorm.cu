@@ -1,0 +1,440 @@
+// The residual's addition and the RMS norm in front of a layer, forward and backward, with the output also as MXFP8 rows.
+//
+//   s = round_to_residual_type(x + r)          (without a residual: s = x)
+//   y = bf16( s * rstd * (w + c) ),            rstd = rsqrt(mean(s^2) + eps)
+// The norm is taken of the stored stream, so that the backward, which reads it back, differentiates the same values:
+//   u = gy * (w + c),   gx = gr = gs + rstd * (u - s * rstd^2 * mean(u * s)),   gw = sum_t gy * s * rstd
+// Quantised rows are those of the MXFP8 row quantiser applied to y, bit for bit, in the packed form that inference calls publish:
+// D bytes E4M3, D / 32 scale bytes, padding to 16 bytes.
+//
+// HBM bound: every value of a row stays in registers between its sum and its use, 2 + 2|4 bytes in and 2 + 2|4 (+ 1.03) out per
+// element.  A row belongs to a warp or to 128, 256 or 512 threads, four (two) 16-byte pieces each.  The gain's gradient is summed
+// over the rows of a block in registers and over the blocks by a second launch, always in the same order.
+#include "quant_common.cuh"
+#include "../../include/dist_moe_b200.h"
+
+namespace dm {
+
+constexpr int kNormMaxVec = 512 * 4;  // 16-byte pieces of bf16 that the register forms hold
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) { unpack8f(*reinterpret_cast<const uint4*>(p), f); }
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ float rounded(const __nv_bfloat16*, float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+__device__ __forceinline__ float rounded(const float*, float v) { return v; }
+
+struct Gain {
+  const void* w;
+  int is_f32;
+  float center;
+  __device__ __forceinline__ void load(int64_t i, float (&g)[8]) const {
+    if (is_f32)
+      load8(static_cast<const float*>(w) + i, g);
+    else
+      load8(static_cast<const __nv_bfloat16*>(w) + i, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] += center;
+  }
+  __device__ __forceinline__ float at(int64_t i) const {
+    return (is_f32 ? static_cast<const float*>(w)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i])) + center;
+  }
+};
+
+struct QuantRows {
+  uint8_t* rows;  // null: not wanted
+  int64_t stride;
+};
+
+// Sum over the kThreads threads that share a row; kThreads > 32 takes the whole block, whose `part` holds a word per warp.
+template <int kThreads>
+__device__ __forceinline__ float row_sum(float v, float* part) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if (kThreads == 32) return v;
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) part[warp] = v;
+  __syncthreads();
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) sum += part[w];
+  return sum;
+}
+
+// The E4M3 bytes and the scale of the block of 32 that four neighbouring lanes hold, 8 values each.  All lanes of a warp call.
+__device__ __forceinline__ void quantise_piece(const uint4& y, int v, bool in, int64_t D, uint8_t* row) {
+  uint32_t m = __vmaxu2(__vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu), __vmaxu2(y.z & 0x7fff7fffu, y.w & 0x7fff7fffu));
+  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  float recip;
+  const uint32_t byte = mxfp8_scale_bits((m >> 16) > (m & 0xffffu) ? m >> 16 : m & 0xffffu, recip);
+  if (!in) return;
+  float f[8];
+  unpack8f(y, f);
+  *reinterpret_cast<uint2*>(row + static_cast<int64_t>(v) * 8) =
+      make_uint2(e4m3x2_scaled(f[0], f[1], recip, recip) | (e4m3x2_scaled(f[2], f[3], recip, recip) << 16),
+                 e4m3x2_scaled(f[4], f[5], recip, recip) | (e4m3x2_scaled(f[6], f[7], recip, recip) << 16));
+  if ((v & 3) == 0) row[D + (v >> 2)] = static_cast<uint8_t>(byte);
+}
+
+// kThreads threads a row, kVec pieces of 8 values a thread.
+template <typename R, bool kResidual, int kThreads, int kVec>
+__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) add_rmsnorm_fwd_kernel(
+    const __nv_bfloat16* __restrict__ x, int64_t x_stride, const R* __restrict__ residual, int64_t r_stride, Gain gain, float eps,
+    int64_t T, int vec, R* __restrict__ sum_out, __nv_bfloat16* __restrict__ y_out, float* __restrict__ rstd_out, QuantRows quant) {
+  __shared__ float part[kThreads / 32];
+  constexpr int kRows = kThreads < 128 ? 128 / kThreads : 1;
+  const int lane = threadIdx.x % kThreads;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kThreads;
+  if (t >= T) return;  // whole warps
+  const int64_t D = static_cast<int64_t>(vec) * 8;
+  float s[kVec][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = i * kThreads + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[i][j] = 0.f;
+    if (v < vec) load8(x + t * x_stride + v * 8, s[i]);
+  }
+  if (kResidual) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = i * kThreads + lane;
+      if (v < vec) {
+        float r[8];
+        load8(residual + t * r_stride + v * 8, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[i][j] = rounded(residual, s[i][j] + r[j]);
+        store8(sum_out + t * D + v * 8, s[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += s[i][j] * s[i][j];
+  const float rstd = rsqrtf(row_sum<kThreads>(ss, part) / static_cast<float>(D) + eps);
+  if (rstd_out != nullptr && lane == 0) rstd_out[t] = rstd;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = i * kThreads + lane;
+    const bool in = v < vec;
+    uint4 y = make_uint4(0, 0, 0, 0);
+    if (in) {
+      float g[8];
+      gain.load(v * 8, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = s[i][j] * rstd * g[j];
+      y = make_uint4(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7]));
+      *reinterpret_cast<uint4*>(y_out + t * D + v * 8) = y;
+    }
+    if (quant.rows != nullptr) quantise_piece(y, v, in, D, quant.rows + t * quant.stride);
+  }
+}
+
+// Rows of any length, stride and alignment, a block each, read twice; not quantised.
+template <typename R, bool kResidual>
+__global__ void __launch_bounds__(256) add_rmsnorm_fwd_any_kernel(
+    const __nv_bfloat16* __restrict__ x, int64_t x_stride, const R* __restrict__ residual, int64_t r_stride, Gain gain, float eps,
+    int64_t T, int64_t D, R* sum_out, __nv_bfloat16* __restrict__ y_out, float* __restrict__ rstd_out) {
+  __shared__ float part[8];
+  const int64_t t = blockIdx.x;
+  float ss = 0.f;
+  for (int64_t i = threadIdx.x; i < D; i += 256) {
+    float v = load1(x + t * x_stride + i);
+    if (kResidual) {
+      v = rounded(residual, v + load1(residual + t * r_stride + i));
+      store1(sum_out + t * D + i, v);
+    }
+    ss += v * v;
+  }
+  const float rstd = rsqrtf(row_sum<256>(ss, part) / static_cast<float>(D) + eps);
+  if (rstd_out != nullptr && threadIdx.x == 0) rstd_out[t] = rstd;
+  for (int64_t i = threadIdx.x; i < D; i += 256) {  // each thread meets its own sums again
+    const float v = kResidual ? load1(sum_out + t * D + i) : load1(x + t * x_stride + i);
+    store1(y_out + t * D + i, v * rstd * gain.at(i));
+  }
+}
+
+// Blocks walk over the rows; `partial` [gridDim.x][D] takes each block's share of the gain's gradient.
+template <typename R, int kThreads, int kVec>
+__global__ void __launch_bounds__(kThreads < 128 ? 128 : kThreads) add_rmsnorm_bwd_kernel(
+    const __nv_bfloat16* __restrict__ grad_y, const R* __restrict__ grad_sum, const R* __restrict__ sum, int64_t sum_stride,
+    Gain gain, const float* __restrict__ rstd_in, int64_t T, int vec, __nv_bfloat16* __restrict__ grad_x,
+    float* __restrict__ grad_residual, float* __restrict__ partial) {
+  constexpr int kRows = kThreads < 128 ? 128 / kThreads : 1;
+  __shared__ float part[2][kThreads / 32];
+  __shared__ float rows[kRows > 1 ? kRows : 1][kRows > 1 ? kThreads * 8 : 1];
+  const int lane = threadIdx.x % kThreads, slot = threadIdx.x / kThreads;
+  const int64_t D = static_cast<int64_t>(vec) * 8;
+  float gw[kVec][8];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) gw[i][j] = 0.f;
+  int it = 0;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kRows + slot; t < T; t += static_cast<int64_t>(gridDim.x) * kRows, ++it) {
+    const float rstd = rstd_in[t];
+    float gy[kVec][8], s[kVec][8];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = i * kThreads + lane;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gy[i][j] = s[i][j] = 0.f;
+      if (v < vec) {
+        load8(grad_y + t * D + v * 8, gy[i]);
+        load8(sum + t * sum_stride + v * 8, s[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = i * kThreads + lane;
+      if (v < vec) {
+        float g[8];
+        gain.load(v * 8, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          gw[i][j] += gy[i][j] * (s[i][j] * rstd);
+          gy[i][j] *= g[j];
+          dot += gy[i][j] * s[i][j];
+        }
+      }
+    }
+    const float mean = row_sum<kThreads>(dot, part[it & 1]) / static_cast<float>(D) * (rstd * rstd);
+    if (grad_x == nullptr && grad_residual == nullptr) continue;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = i * kThreads + lane;
+      if (v < vec) {
+        float g[8];
+        if (grad_sum != nullptr)
+          load8(grad_sum + t * D + v * 8, g);
+        else
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[j] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] += rstd * (gy[i][j] - s[i][j] * mean);
+        if (grad_x != nullptr) store8(grad_x + t * D + v * 8, g);
+        if (grad_residual != nullptr) store8(grad_residual + t * D + v * 8, g);
+      }
+    }
+  }
+  if (partial == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = i * kThreads + lane;
+    if (kRows > 1) {  // the block's warps in order
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rows[slot][lane * 8 + j] = gw[i][j];
+      __syncthreads();
+      if (slot == 0)
+#pragma unroll
+        for (int r = 1; r < kRows; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) gw[i][j] += rows[r][lane * 8 + j];
+    }
+    if (slot == 0 && v < vec) store8(partial + blockIdx.x * D + v * 8, gw[i]);
+  }
+}
+
+template <typename R>
+__global__ void __launch_bounds__(256) add_rmsnorm_bwd_any_kernel(
+    const __nv_bfloat16* __restrict__ grad_y, const R* __restrict__ grad_sum, const R* __restrict__ sum, int64_t sum_stride,
+    Gain gain, const float* __restrict__ rstd_in, int64_t T, int64_t D, __nv_bfloat16* __restrict__ grad_x,
+    float* __restrict__ grad_residual, float* partial) {
+  __shared__ float part[2][8];
+  int it = 0;
+  for (int64_t t = blockIdx.x; t < T; t += gridDim.x, ++it) {
+    const float rstd = rstd_in[t];
+    float dot = 0.f;
+    for (int64_t i = threadIdx.x; i < D; i += 256) {
+      const float g = load1(grad_y + t * D + i), s = load1(sum + t * sum_stride + i);
+      dot += g * gain.at(i) * s;
+      if (partial != nullptr) {  // a thread's own columns
+        float* own = partial + blockIdx.x * D + i;
+        *own = (it == 0 ? 0.f : *own) + g * (s * rstd);
+      }
+    }
+    const float mean = row_sum<256>(dot, part[it & 1]) / static_cast<float>(D) * (rstd * rstd);
+    if (grad_x == nullptr && grad_residual == nullptr) continue;
+    for (int64_t i = threadIdx.x; i < D; i += 256) {
+      const float g = load1(grad_y + t * D + i) * gain.at(i), s = load1(sum + t * sum_stride + i);
+      const float v = (grad_sum != nullptr ? load1(grad_sum + t * D + i) : 0.f) + rstd * (g - s * mean);
+      if (grad_x != nullptr) store1(grad_x + t * D + i, v);
+      if (grad_residual != nullptr) grad_residual[t * D + i] = v;
+    }
+  }
+}
+
+// Sum of the blocks' shares: 32 columns a block, eight warps that take every eighth share and meet in order.
+template <typename W>
+__global__ void __launch_bounds__(256) add_rmsnorm_gain_kernel(const float* __restrict__ partial, int shares, int64_t D, W* __restrict__ out) {
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float sum = 0.f;
+  if (c < D)
+#pragma unroll 4
+    for (int b = warp; b < shares; b += 8) sum += partial[b * D + c];
+  part[warp][lane] = sum;
+  __syncthreads();
+  if (warp != 0 || c >= D) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) sum += part[w][lane];
+  store1(out + c, sum);
+}
+
+// Packed MXFP8 rows back to bf16, exactly (4 significant bits times a power of two).
+__global__ void __launch_bounds__(256) mxfp8_dequant_rows_kernel(const uint8_t* __restrict__ rows, int64_t stride, int64_t T, int vec,
+                                                                 uint4* __restrict__ out) {
+  const int64_t n = T * vec, step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x; i < n; i += step) {
+    const int64_t t = i / vec;
+    const int v = static_cast<int>(i - t * vec);
+    const uint8_t* row = rows + t * stride;
+    const uint2 q = *reinterpret_cast<const uint2*>(row + v * 8);
+    const uint32_t byte = row[vec * 8 + (v >> 2)];
+    const float scale = byte == 0xffu ? __int_as_float(0x7fc00000) : byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t two = (j < 2 ? q.x : q.y) >> (16 * (j & 1));
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      w[j] = pack_bf16x2(f.x * scale, f.y * scale);
+    }
+    out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Blocks of the backward: as many as the device holds at once, so that few shares of the gain's gradient are left.
+static int64_t norm_bwd_blocks(int64_t T, int64_t D) {
+  const int64_t rows = D <= 1024 ? 4 : 1;
+  const int64_t most = grid_cap(D <= 4096 ? 4 : D <= 8192 ? 2 : 1);
+  const int64_t blocks = ceil_div64(T, rows);
+  return blocks < most ? blocks : most;
+}
+
+}  // namespace dm
+
+using namespace dm;
+
+template <typename R, bool kResidual>
+static int add_rmsnorm_fwd(const void* x, int64_t x_stride, const void* residual, int64_t r_stride, const Gain& gain, float eps,
+                           int64_t T, int64_t D, void* sum_out, void* y_out, float* rstd_out, const QuantRows& quant, cudaStream_t st) {
+  const auto* xp = static_cast<const __nv_bfloat16*>(x);
+  const auto* rp = static_cast<const R*>(residual);
+  auto* sp = static_cast<R*>(sum_out);
+  auto* yp = static_cast<__nv_bfloat16*>(y_out);
+  const bool vectors = D % 8 == 0 && D / 8 <= kNormMaxVec && aligned16(x) && x_stride % 8 == 0 && aligned16(gain.w) && aligned16(y_out) &&
+                       (!kResidual || (aligned16(residual) && aligned16(sum_out) && r_stride % 8 == 0));
+  if (!vectors) {
+    if (quant.rows != nullptr) return kRcUnsupportedShape;
+    add_rmsnorm_fwd_any_kernel<R, kResidual><<<static_cast<unsigned>(T), 256, 0, st>>>(xp, x_stride, rp, r_stride, gain, eps, T, D, sp, yp, rstd_out);
+    return static_cast<int>(cudaGetLastError());
+  }
+  auto run = [&](auto kernel, int threads) {
+    const int rows = threads < 128 ? 128 / threads : 1;
+    kernel<<<static_cast<unsigned>(ceil_div64(T, rows)), threads < 128 ? 128 : threads, 0, st>>>(
+        xp, x_stride, rp, r_stride, gain, eps, T, static_cast<int>(D / 8), sp, yp, rstd_out, quant);
+    return static_cast<int>(cudaGetLastError());
+  };
+  if (D <= 1024) return run(add_rmsnorm_fwd_kernel<R, kResidual, 32, 4>, 32);
+  if (D <= 2048) return run(add_rmsnorm_fwd_kernel<R, kResidual, 128, 2>, 128);
+  if (D <= 4096) return run(add_rmsnorm_fwd_kernel<R, kResidual, 128, 4>, 128);
+  if (D <= 8192) return run(add_rmsnorm_fwd_kernel<R, kResidual, 256, 4>, 256);
+  return run(add_rmsnorm_fwd_kernel<R, kResidual, 512, 4>, 512);
+}
+
+extern "C" int dm_add_rmsnorm_fwd(const void* x, int64_t x_stride, const void* residual, int residual_is_f32, int64_t residual_stride,
+                                  const void* weight, int weight_is_f32, float gain_center, float eps, int64_t T, int64_t D,
+                                  void* sum_out, void* y_out, float* rstd_out, void* rows_out, int64_t row_stride, void* stream) {
+  if (T < 0 || T > 0x7fffffff || D <= 0 || x_stride < 0 || residual_stride < 0) return kRcBadArg;
+  if (T == 0) return kRcOk;
+  if (!x || !weight || !y_out || (residual != nullptr) != (sum_out != nullptr)) return kRcBadArg;
+  if (rows_out != nullptr && (D % 32 != 0 || row_stride % 16 != 0 || row_stride < D + D / 32 || !aligned16(rows_out)))
+    return kRcUnsupportedShape;
+  const Gain gain{weight, weight_is_f32, gain_center};
+  const QuantRows quant{static_cast<uint8_t*>(rows_out), row_stride};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (residual == nullptr)
+    return add_rmsnorm_fwd<__nv_bfloat16, false>(x, x_stride, nullptr, 0, gain, eps, T, D, nullptr, y_out, rstd_out, quant, st);
+  if (residual_is_f32)
+    return add_rmsnorm_fwd<float, true>(x, x_stride, residual, residual_stride, gain, eps, T, D, sum_out, y_out, rstd_out, quant, st);
+  return add_rmsnorm_fwd<__nv_bfloat16, true>(x, x_stride, residual, residual_stride, gain, eps, T, D, sum_out, y_out, rstd_out, quant, st);
+}
+
+extern "C" int64_t dm_add_rmsnorm_shares(int64_t T, int64_t D) { return T <= 0 || D <= 0 ? 0 : norm_bwd_blocks(T, D); }
+
+template <typename R>
+static int add_rmsnorm_bwd(const void* grad_y, const void* grad_sum, const void* sum, int64_t sum_stride, const Gain& gain,
+                           const float* rstd, int64_t T, int64_t D, void* grad_x, float* grad_residual, float* partial, cudaStream_t st) {
+  const auto* gy = static_cast<const __nv_bfloat16*>(grad_y);
+  const auto* gs = static_cast<const R*>(grad_sum);
+  const auto* sp = static_cast<const R*>(sum);
+  auto* gx = static_cast<__nv_bfloat16*>(grad_x);
+  const int blocks = static_cast<int>(norm_bwd_blocks(T, D));
+  const bool vectors = D % 8 == 0 && D / 8 <= kNormMaxVec && aligned16(gy) && aligned16(gs) && aligned16(sp) && sum_stride % 8 == 0 &&
+                       aligned16(gain.w) && aligned16(gx) && aligned16(grad_residual) && aligned16(partial);
+  if (!vectors) {
+    add_rmsnorm_bwd_any_kernel<R><<<blocks, 256, 0, st>>>(gy, gs, sp, sum_stride, gain, rstd, T, D, gx, grad_residual, partial);
+    return static_cast<int>(cudaGetLastError());
+  }
+  auto run = [&](auto kernel, int threads) {
+    kernel<<<blocks, threads < 128 ? 128 : threads, 0, st>>>(gy, gs, sp, sum_stride, gain, rstd, T, static_cast<int>(D / 8), gx,
+                                                             grad_residual, partial);
+    return static_cast<int>(cudaGetLastError());
+  };
+  if (D <= 1024) return run(add_rmsnorm_bwd_kernel<R, 32, 4>, 32);
+  if (D <= 2048) return run(add_rmsnorm_bwd_kernel<R, 128, 2>, 128);
+  if (D <= 4096) return run(add_rmsnorm_bwd_kernel<R, 128, 4>, 128);
+  if (D <= 8192) return run(add_rmsnorm_bwd_kernel<R, 256, 4>, 256);
+  return run(add_rmsnorm_bwd_kernel<R, 512, 4>, 512);
+}
+
+extern "C" int dm_add_rmsnorm_bwd(const void* grad_y, const void* grad_sum, const void* sum, int sum_is_f32, int64_t sum_stride,
+                                  const void* weight, int weight_is_f32, float gain_center, const float* rstd, int64_t T, int64_t D,
+                                  void* grad_x, float* grad_residual, float* partial, void* grad_weight, void* stream) {
+  if (T <= 0 || T > 0x7fffffff || D <= 0 || sum_stride < 0) return kRcBadArg;
+  if (!grad_y || !sum || !weight || !rstd || (partial != nullptr) != (grad_weight != nullptr)) return kRcBadArg;
+  const Gain gain{weight, weight_is_f32, gain_center};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rc = sum_is_f32
+                     ? add_rmsnorm_bwd<float>(grad_y, grad_sum, sum, sum_stride, gain, rstd, T, D, grad_x, grad_residual, partial, st)
+                     : add_rmsnorm_bwd<__nv_bfloat16>(grad_y, grad_sum, sum, sum_stride, gain, rstd, T, D, grad_x, grad_residual, partial, st);
+  if (rc != 0 || grad_weight == nullptr) return rc;
+  const unsigned columns = static_cast<unsigned>(ceil_div64(D, 32));
+  const int shares = static_cast<int>(norm_bwd_blocks(T, D));
+  if (weight_is_f32)
+    add_rmsnorm_gain_kernel<float><<<columns, 256, 0, st>>>(partial, shares, D, static_cast<float*>(grad_weight));
+  else
+    add_rmsnorm_gain_kernel<__nv_bfloat16><<<columns, 256, 0, st>>>(partial, shares, D, static_cast<__nv_bfloat16*>(grad_weight));
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int dm_dequant_mxfp8_rows(const void* rows, int64_t row_stride, int64_t T, int64_t D, void* out, void* stream) {
+  if (T < 0 || D <= 0 || D % 32 != 0 || row_stride % 16 != 0 || row_stride < D + D / 32) return kRcBadArg;
+  if (T == 0) return kRcOk;
+  if (!rows || !out || !aligned16(rows) || !aligned16(out)) return kRcBadArg;
+  const int64_t blocks = ceil_div64(T * (D / 8), 256);
+  mxfp8_dequant_rows_kernel<<<static_cast<int>(blocks < grid_cap(8) ? blocks : grid_cap(8)), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(rows), row_stride, T, static_cast<int>(D / 8), static_cast<uint4*>(out));
+  return static_cast<int>(cudaGetLastError());
+}

@@ -53,4 +53,29 @@ __device__ __forceinline__ float amax_from_bf16_bits(uint32_t bits15) {
   return bits15 > 0x7f80u ? __int_as_float(0x7f800000) : __uint_as_float(bits15 << 16);
 }
 
+// Scale byte and reciprocal of a block of bf16 values from the low 15 bits of its largest magnitude: the byte that
+// mxfp8_scale computes through fp32, in integers.  amax / 448 <= 2^(b - 127) holds for bf16 exactly when the
+// (exponent, mantissa) pair is <= (b + 8, 0x60), 448 being 1.75 * 2^8; bytes below 0 are 0, a non-finite block is 0xFF.
+__device__ __forceinline__ uint32_t mxfp8_scale_bits(uint32_t bits15, float& recip) {
+  const int b = static_cast<int>((bits15 + 0x1fu) >> 7) - 8;
+  const uint32_t byte = bits15 >= 0x7f80u ? 0xffu : static_cast<uint32_t>(b > 0 ? b : 0);
+  recip = byte == 0xffu ? __int_as_float(0x7fc00000) : __uint_as_float((254u - byte) << 23);
+  return byte;
+}
+
+// Products of two packed fp32 pairs (one instruction), as two E4M3 bytes.
+__device__ __forceinline__ uint32_t e4m3x2_scaled(float lo, float hi, float r_lo, float r_hi) {
+  float a, b;
+  asm("{\n\t"
+      ".reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t"
+      "}\n"
+      : "=f"(a), "=f"(b)
+      : "f"(lo), "f"(hi), "f"(r_lo), "f"(r_hi));
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
 }  // namespace dm

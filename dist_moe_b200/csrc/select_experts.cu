@@ -1,0 +1,456 @@
+// Expert ids and scores of every token from the router's logits, forward and backward.
+//
+//   p = softmax(l) over the experts, or sigmoid(l);   c = p + b (b: optional bias, for the choice alone)
+//   with groups: a group's value is the sum of its one or two largest c, and the experts of the `kept` best groups remain
+//   ids = the K largest c in falling order, equal values by index;   v_k = p[ids_k]
+//   score_k = scale * v_k, or scale * v_k / sum_j v_j
+// An expert whose logit or c is -inf or NaN is not chosen (a NaN logit counts as -inf); where fewer than K are left, and for masked
+// tokens, ids are -1 and scores 0, which is how the routed experts take a route that goes nowhere.  +inf logits share the softmax.
+//
+// The choice is the one of 64-bit arithmetic.  Without a bias p is monotone in l, so experts are compared by their logits.  Otherwise c
+// in 32 bits carries an error of a few units in the last place; a row in which two values that decide something lie nearer than that
+// is chosen once more in 64 bits (under one row in a hundred of normally distributed logits).
+//
+// Backward, w_k = v_k / sum v, g_k = scale * grad_k:
+//   softmax            dl_i = p_i (g_i [i chosen] - sum_k p_k g_k)
+//   sigmoid            dl_k = g_k p_k (1 - p_k)
+//   softmax, normalised  dl_k = w_k (g_k - sum_j w_j g_j);   sigmoid, normalised: the same times 1 - p_k
+//
+// A warp per token: its logits sit in registers, expert 32 j + lane in register j; each of the K rounds is two warp reductions and a
+// rescan of the winning lane's registers.
+#include <type_traits>
+
+#include "common.cuh"
+#include "../../include/dist_moe_b200.h"
+
+namespace dm {
+
+constexpr int kSelectWarps = 4;
+
+struct SelectParams {
+  const void* logits;
+  int64_t stride;  // elements between rows
+  int64_t T;
+  int E, K, groups, kept, group_top;
+  int sigmoid, renormalize;
+  float scale;
+  const float* bias;            // null: none
+  const unsigned char* mask;    // null: every token is live
+  void* ids;
+  void* scores;
+  int ids_are_int64, scores_are_bf16;
+};
+
+__device__ __forceinline__ float select_load(const float* p) { return *p; }
+__device__ __forceinline__ float select_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void select_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void select_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ V warp_sum(V v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// Floats as unsigned words of the same order; 0 for what cannot be chosen.  Adding zero makes -0 equal to +0.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (!(v > neg_inf())) return 0;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b ^ (static_cast<int32_t>(b) < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ (static_cast<int32_t>(k) < 0 ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ uint64_t order_key(double v) {
+  if (!(v > static_cast<double>(neg_inf()))) return 0;
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+  return b ^ (static_cast<int64_t>(b) < 0 ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ uint32_t warp_max_key(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
+__device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const uint64_t o = __shfl_xor_sync(0xffffffffu, k, d);
+    k = o > k ? o : k;
+  }
+  return k;
+}
+
+__device__ __forceinline__ float exp_v(float x) { return expf(x); }
+__device__ __forceinline__ double exp_v(double x) { return exp(x); }
+
+// What the softmax's exponential is taken of: +inf logits, which are the largest then, share it.
+template <typename V>
+__device__ __forceinline__ V below(float l, float top) {
+  return l == top ? V(0) : V(l) - V(top);
+}
+
+// Two largest of two pairs (falling); keys, 0 = nothing.
+template <typename V>
+struct Top2 {
+  V first, second;  // -inf: nothing
+  __device__ __forceinline__ void add(V v) {
+    if (v > first) {
+      second = first;
+      first = v;
+    } else if (v > second) {
+      second = v;
+    }
+  }
+};
+
+// The choice in V arithmetic.  c(e) is the value of expert e for the comparison between groups (and between experts where `by_value`);
+// `keys` are the experts' keys in the calling warp's registers.  Returns whether two values that decide something were nearer than the
+// error of V allows; the chosen index of round k ends up in lane k.
+template <int kPer, typename Key, typename V>
+__device__ __forceinline__ bool choose(Key (&keys)[kPer], const V* values, V tolerance, bool check, const SelectParams& p, int lane,
+                                       int& chosen) {
+  bool near = false;
+  const V nothing = static_cast<V>(neg_inf());
+  if (p.groups > 1) {
+    // lanes_per lanes look through a group; `values` is this warp's row of shared memory
+    const int size = p.E / p.groups;
+    int lanes_per = 32;
+    while (32 / lanes_per < p.groups) lanes_per >>= 1;
+    const int group = lane / lanes_per, sub = lane % lanes_per;
+    Top2<V> best{nothing, nothing};
+    if (group < p.groups)
+      for (int i = sub; i < size; i += lanes_per) best.add(values[group * size + i]);
+    for (int d = 1; d < lanes_per; d <<= 1) {
+      const V a = __shfl_xor_sync(0xffffffffu, best.first, d), b = __shfl_xor_sync(0xffffffffu, best.second, d);
+      best.add(a);
+      best.add(b);
+    }
+    const V value = p.group_top == 2 && best.second > nothing ? best.first + best.second : best.first;
+    // rank of this lane's group: groups of larger value, or of equal value and lower index
+    int rank = 0;
+    V above = static_cast<V>(-neg_inf()), under = nothing;  // nearest values on the other side of the border
+    for (int g = 0; g < p.groups; ++g) {
+      const V other = __shfl_sync(0xffffffffu, value, g * lanes_per);
+      if (other > value || (other == value && g < group)) ++rank;
+    }
+    const bool keep = group < p.groups && rank < p.kept;
+    if (check && p.kept < p.groups) {
+      V span = group < p.groups && best.first > nothing ? fabs(best.first) + (p.group_top == 2 && best.second > nothing ? fabs(best.second) : V(0)) : V(0);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) {
+        const V other = __shfl_xor_sync(0xffffffffu, span, d);
+        span = other > span ? other : span;
+      }
+      for (int g = 0; g < p.groups; ++g) {
+        const V other = __shfl_sync(0xffffffffu, value, g * lanes_per);
+        const bool kept = __shfl_sync(0xffffffffu, keep ? 1 : 0, g * lanes_per) != 0;
+        if (kept)
+          above = other < above ? other : above;
+        else
+          under = other > under ? other : under;
+      }
+      // sums of two values each: two errors on either side.  Written so that infinities on both sides count as near.
+      near = under > nothing && !(above - under > 4 * tolerance * (1 + span));
+    }
+    uint32_t kept_groups = __ballot_sync(0xffffffffu, keep && sub == 0);  // bit group * lanes_per
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int e = 32 * j + lane;
+      if (e < p.E && !(kept_groups >> (e / size * lanes_per) & 1)) keys[j] = 0;
+    }
+  }
+  Key mine = 0;
+  int at = 0;
+  auto rescan = [&] {
+    mine = keys[0];
+    at = 0;
+#pragma unroll
+    for (int j = 1; j < kPer; ++j)
+      if (keys[j] > mine) {
+        mine = keys[j];
+        at = j;
+      }
+  };
+  rescan();
+  chosen = -1;
+  Key last = 0;
+  for (int k = 0; k < p.K + (check ? 1 : 0); ++k) {
+    const Key top = warp_max_key(mine);
+    if (top == 0) break;
+    const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, mine == top ? static_cast<uint32_t>(32 * at + lane) : 0xffffffffu));
+    if (check && k > 0 && sizeof(Key) == 4) {
+      const float a = key_value(static_cast<uint32_t>(last)), b = key_value(static_cast<uint32_t>(top));
+      near = near || !(a - b > 2.0f * static_cast<float>(tolerance) * (1.0f + fabsf(a)));
+    }
+    last = top;
+    if (k < p.K && lane == k) chosen = e;
+    if (lane == (e & 31)) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (j == (e >> 5)) keys[j] = 0;
+      rescan();
+    }
+  }
+  return near;
+}
+
+// The row in 64 bits: its values go through `values64`, shared memory of this warp (E doubles).
+template <int kPer, typename L>
+__device__ __noinline__ int choose_again(const SelectParams& p, const L* row, float top, double* values64, int lane) {
+  double z = 1.0;
+  if (!p.sigmoid) {
+    z = 0.0;
+    for (int e = lane; e < p.E; e += 32) {
+      const float l = select_load(row + e);
+      if (l > neg_inf()) z += exp(below<double>(l, top));
+    }
+    z = warp_sum(z);
+  }
+  uint64_t keys[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int e = 32 * j + lane;
+    keys[j] = 0;
+    if (e < p.E) {
+      const float l = select_load(row + e);
+      double c = static_cast<double>(neg_inf());
+      if (l > neg_inf()) c = (p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l))) : exp(below<double>(l, top)) / z);
+      if (p.bias != nullptr && l > neg_inf()) c += static_cast<double>(p.bias[e]);
+      keys[j] = order_key(c);
+      if (keys[j] == 0) c = static_cast<double>(neg_inf());
+      // without a bias logits are compared, as in the 32-bit form
+      if (p.bias == nullptr && keys[j] != 0) keys[j] = order_key(static_cast<double>(l));
+      values64[e] = c;
+    }
+  }
+  __syncwarp();
+  int chosen;
+  choose<kPer, uint64_t, double>(keys, values64, 0.0, false, p, lane, chosen);
+  return chosen;
+}
+
+template <int kPer, typename L>
+__global__ void __launch_bounds__(32 * kSelectWarps) select_experts_kernel(const SelectParams p) {
+  extern __shared__ double select_smem[];  // a row of E doubles per warp where values are compared
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kSelectWarps + warp;
+  if (t >= p.T) return;
+  const L* row = static_cast<const L*>(p.logits) + t * p.stride;
+  int chosen = -1;
+  float score = 0.f;
+  if (p.mask == nullptr || p.mask[t] != 0) {
+    float l[kPer];
+    float top = neg_inf();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int e = 32 * j + lane;
+      l[j] = e < p.E ? select_load(row + e) : neg_inf();
+      if (!(l[j] > neg_inf())) l[j] = neg_inf();  // NaN
+      top = fmaxf(top, l[j]);
+    }
+    const bool by_value = p.bias != nullptr;
+    const bool values = by_value || p.groups > 1;
+    float z = 1.f;
+    if (!p.sigmoid) {
+      top = warp_max(top);
+      if (values || !p.renormalize) {
+        z = 0.f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (l[j] > neg_inf()) z += expf(below<float>(l[j], top));
+        z = warp_sum(z);
+      }
+    }
+    double* row64 = select_smem + static_cast<int64_t>(warp) * p.E;
+    float* row32 = reinterpret_cast<float*>(row64);
+    uint32_t keys[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int e = 32 * j + lane;
+      keys[j] = order_key(l[j]);
+      if (values && e < p.E) {
+        float c = neg_inf();
+        if (keys[j] != 0) {
+          c = p.sigmoid ? 1.0f / (1.0f + expf(-l[j])) : expf(below<float>(l[j], top)) / z;
+          if (by_value) c += p.bias[e];
+          if (!(c > neg_inf())) c = neg_inf();
+          if (by_value) keys[j] = order_key(c);
+        }
+        if (p.groups > 1) row32[e] = c;
+      }
+    }
+    if (p.groups > 1) __syncwarp();
+    // Error of c relative to 1 + |c|.  Sigmoid: exponential (1 unit in the last place, halved by p (1 - p) <= 1/4 in absolute terms),
+    // sum, quotient and the bias' addition, half a unit each: under 2^-22.  Softmax: the sum of up to 1024 terms as well, 37 roundings
+    // of half a unit: under 2^-18.
+    const float tolerance = p.sigmoid ? 0x1p-22f : 0x1p-18f;
+    bool near;
+    if (by_value) {
+      near = choose<kPer, uint32_t, float>(keys, row32, tolerance, true, p, lane, chosen);
+    } else {
+      // experts by their logits, exactly; groups by values
+      SelectParams q = p;
+      near = false;
+      if (p.groups > 1) {
+        uint32_t copy[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) copy[j] = keys[j];
+        q.K = 0;  // the groups' border alone
+        near = choose<kPer, uint32_t, float>(copy, row32, tolerance, true, q, lane, chosen);
+      }
+      choose<kPer, uint32_t, float>(keys, row32, tolerance, false, p, lane, chosen);
+    }
+    if (values && near) {
+      __syncwarp();
+      chosen = choose_again<kPer, L>(p, row, top, row64, lane);
+    }
+    // lane k: the score of the k-th
+    const bool have = lane < p.K && chosen >= 0;
+    const float lk = have ? select_load(row + chosen) : neg_inf();
+    if (p.renormalize) {
+      // relative to the largest chosen logit, so that nothing underflows together: p_k = e^(l - m) (softmax) or e^(l - m) / (1 + e^l)
+      float m = warp_max(lk);
+      if (p.sigmoid && m > 0.f) m = 0.f;
+      float v = 0.f;
+      if (have) v = !p.sigmoid ? expf(below<float>(lk, m)) : lk >= 0.f ? 1.0f / (1.0f + expf(-lk)) : expf(below<float>(lk, m)) / (1.0f + expf(lk));
+      const float sum = warp_sum(v);
+      if (have) score = p.scale * (v / sum);
+    } else if (have) {
+      score = p.scale * (p.sigmoid ? 1.0f / (1.0f + expf(-lk)) : expf(below<float>(lk, top)) / z);
+    }
+  }
+  if (lane < p.K) {
+    const int64_t at = t * p.K + lane;
+    if (p.ids_are_int64)
+      static_cast<int64_t*>(p.ids)[at] = chosen;
+    else
+      static_cast<int32_t*>(p.ids)[at] = chosen;
+    if (p.scores_are_bf16)
+      static_cast<__nv_bfloat16*>(p.scores)[at] = __float2bfloat16_rn(score);
+    else
+      static_cast<float*>(p.scores)[at] = score;
+  }
+}
+
+struct SelectGradParams {
+  const void* logits;
+  int64_t stride, T;
+  int E, K, sigmoid, renormalize;
+  float scale;
+  const void* ids;
+  const void* grad_scores;
+  int ids_are_int64, scores_are_bf16;
+  void* grad_logits;  // [T, E]
+};
+
+template <typename L>
+__global__ void __launch_bounds__(32 * kSelectWarps) select_experts_bwd_kernel(const SelectGradParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kSelectWarps + (threadIdx.x >> 5);
+  if (t >= p.T) return;
+  const L* row = static_cast<const L*>(p.logits) + t * p.stride;
+  L* out = static_cast<L*>(p.grad_logits) + t * p.E;
+  int id = -1;
+  float g = 0.f, l = neg_inf();
+  if (lane < p.K) {
+    const int64_t at = t * p.K + lane;
+    id = static_cast<int>(p.ids_are_int64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<const int32_t*>(p.ids)[at]);
+    if (id >= p.E) id = -1;
+    if (id >= 0) {
+      l = select_load(row + id);
+      g = p.scale * (p.scores_are_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.grad_scores)[at])
+                                       : static_cast<const float*>(p.grad_scores)[at]);
+    }
+  }
+  const bool have = id >= 0;
+  float own = 0.f;  // gradient of the lane's chosen logit
+  if (p.renormalize || p.sigmoid) {
+    const float q = have ? 1.0f / (1.0f + expf(l)) : 0.f;  // 1 - sigmoid
+    if (p.renormalize) {
+      float m = warp_max(l);
+      if (p.sigmoid && m > 0.f) m = 0.f;
+      float v = 0.f;
+      if (have) v = !p.sigmoid ? expf(below<float>(l, m)) : l >= 0.f ? 1.0f / (1.0f + expf(-l)) : expf(below<float>(l, m)) * q;
+      const float sum = warp_sum(v);
+      const float w = have ? v / sum : 0.f;
+      const float mean = warp_sum(w * g);
+      own = w * (g - mean) * (p.sigmoid ? q : 1.0f);
+    } else if (have) {
+      own = g * q / (1.0f + expf(-l));
+    }
+    for (int e = lane; e < p.E; e += 32) select_store(out + e, 0.f);
+  } else {
+    float top = neg_inf();
+    for (int e = lane; e < p.E; e += 32) {
+      const float x = select_load(row + e);
+      if (x > top) top = x;
+    }
+    top = warp_max(top);
+    float z = 0.f;
+    for (int e = lane; e < p.E; e += 32) {
+      const float x = select_load(row + e);
+      if (x > neg_inf()) z += expf(below<float>(x, top));
+    }
+    z = warp_sum(z);
+    const float v = have ? expf(below<float>(l, top)) / z : 0.f;
+    const float dot = warp_sum(v * g);
+    own = v * (g - dot);
+    for (int e = lane; e < p.E; e += 32) {
+      const float x = select_load(row + e);
+      select_store(out + e, x > neg_inf() ? -dot * (expf(below<float>(x, top)) / z) : 0.f);
+    }
+  }
+  __syncwarp();  // the chosen ones over what was just written
+  if (have) select_store(out + id, own);
+}
+
+}  // namespace dm
+
+using namespace dm;
+
+constexpr int kSelectMaxExperts = 1024;
+
+extern "C" int dm_select_experts(const void* logits, int logits_are_bf16, int64_t stride, int64_t T, int E, int K, int sigmoid,
+                                 const float* bias, int groups, int kept, int group_top, int renormalize, float scale,
+                                 const void* mask, void* ids, int ids_are_int64, void* scores, int scores_are_bf16, void* stream) {
+  if (T < 0 || T > (int64_t{1} << 32) || E <= 0 || K <= 0 || K > 32 || K > E || stride < 0) return kRcBadArg;
+  if (groups <= 0 || groups > 32 || E % groups != 0 || kept <= 0 || kept > groups || (group_top != 1 && group_top != 2)) return kRcBadArg;
+  if (E > kSelectMaxExperts) return kRcTooLarge;
+  if (T == 0) return kRcOk;
+  if (!logits || !ids || !scores) return kRcBadArg;
+  SelectParams p{logits, stride, T, E, K, groups, kept, group_top, sigmoid, renormalize, scale, bias,
+                 static_cast<const unsigned char*>(mask), ids, scores, ids_are_int64, scores_are_bf16};
+  const unsigned blocks = static_cast<unsigned>(ceil_div64(T, kSelectWarps));
+  const size_t smem = bias != nullptr || groups > 1 ? static_cast<size_t>(kSelectWarps) * E * sizeof(double) : 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto run = [&](auto per) {
+    if (logits_are_bf16)
+      select_experts_kernel<decltype(per)::value, __nv_bfloat16><<<blocks, 32 * kSelectWarps, smem, st>>>(p);
+    else
+      select_experts_kernel<decltype(per)::value, float><<<blocks, 32 * kSelectWarps, smem, st>>>(p);
+    return static_cast<int>(cudaGetLastError());
+  };
+  if (E <= 32) return run(std::integral_constant<int, 1>{});
+  if (E <= 64) return run(std::integral_constant<int, 2>{});
+  if (E <= 128) return run(std::integral_constant<int, 4>{});
+  if (E <= 256) return run(std::integral_constant<int, 8>{});
+  if (E <= 512) return run(std::integral_constant<int, 16>{});
+  return run(std::integral_constant<int, 32>{});
+}
+
+extern "C" int dm_select_experts_bwd(const void* logits, int logits_are_bf16, int64_t stride, int64_t T, int E, int K, int sigmoid,
+                                     int renormalize, float scale, const void* ids, int ids_are_int64, const void* grad_scores,
+                                     int scores_are_bf16, void* grad_logits, void* stream) {
+  if (T < 0 || T > (int64_t{1} << 32) || E <= 0 || K <= 0 || K > 32 || K > E || stride < 0) return kRcBadArg;
+  if (E > kSelectMaxExperts) return kRcTooLarge;
+  if (T == 0) return kRcOk;
+  if (!logits || !ids || !grad_scores || !grad_logits) return kRcBadArg;
+  const SelectGradParams p{logits, stride, T, E, K, sigmoid, renormalize, scale, ids, grad_scores, ids_are_int64, scores_are_bf16, grad_logits};
+  const unsigned blocks = static_cast<unsigned>(ceil_div64(T, kSelectWarps));
+  if (logits_are_bf16)
+    select_experts_bwd_kernel<__nv_bfloat16><<<blocks, 32 * kSelectWarps, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  else
+    select_experts_bwd_kernel<float><<<blocks, 32 * kSelectWarps, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}

@@ -682,6 +682,50 @@ int dm_bf16_backward(const dm_layer_context* context, const dm_layer_call* call,
 int dm_mxfp8_forward(const dm_layer_context* context, const dm_layer_call* call, uint32_t steps, int32_t* report, void* stream);
 int dm_mxfp8_backward(const dm_layer_context* context, const dm_layer_call* call, uint32_t steps, int32_t* report, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Around the routed experts of a layer.
+ *
+ * dm_add_rmsnorm_fwd: sum = x + residual, rounded to the residual's type (bf16 or fp32), y = bf16(sum * rstd * (weight +
+ * gain_center)), rstd = rsqrt(mean(sum^2) + eps).  x is bf16; rows of x and of the residual start `*_stride` elements apart.  Without
+ * a residual (NULL, as sum_out then) x itself is normalised.  rstd_out [T] and rows_out may be NULL.  rows_out: y as MXFP8 in the
+ * packed form that inference calls publish, rows of `row_stride` bytes [D bytes E4M3 | D / 32 scales E8M0 | padding]; D % 32 == 0
+ * and 16-byte aligned operands, D <= 16384.
+ * dm_add_rmsnorm_bwd: grad_x (bf16) and grad_residual (fp32) both take the gradient of `sum`; either may be NULL, and so may
+ * grad_sum.  partial: fp32 [dm_add_rmsnorm_shares(T, D)][D], given together with grad_weight (of the weight's type) or NULL.
+ * dm_dequant_mxfp8_rows: packed rows as bf16 [T, D].
+ * ------------------------------------------------------------------------- */
+int dm_add_rmsnorm_fwd(const void* x, int64_t x_stride, const void* residual, int residual_is_f32, int64_t residual_stride,
+                       const void* weight, int weight_is_f32, float gain_center, float eps, int64_t T, int64_t D, void* sum_out,
+                       void* y_out, float* rstd_out, void* rows_out, int64_t row_stride, void* stream);
+int64_t dm_add_rmsnorm_shares(int64_t T, int64_t D);
+int dm_add_rmsnorm_bwd(const void* grad_y, const void* grad_sum, const void* sum, int sum_is_f32, int64_t sum_stride,
+                       const void* weight, int weight_is_f32, float gain_center, const float* rstd, int64_t T, int64_t D,
+                       void* grad_x, float* grad_residual, float* partial, void* grad_weight, void* stream);
+int dm_dequant_mxfp8_rows(const void* rows, int64_t row_stride, int64_t T, int64_t D, void* out_bf16, void* stream);
+
+/* dm_select_experts: ids and scores [T, K] from logits [T, E] (rows `stride` elements apart).  p = softmax or sigmoid, c = p + bias
+ * (fp32 [E] or NULL); the `kept` of `groups` groups with the largest sums of their group_top (1 or 2) largest c remain; the K largest
+ * c, equal ones by index, as in 64-bit arithmetic; score = scale * p, normalised over the K where asked.  -inf and NaN are not
+ * chosen; missing choices and tokens whose mask byte is 0 get id -1 and score 0.  E <= 1024, K <= 32, groups <= 32.
+ * dm_select_experts_bwd: the logits' gradient [T, E], of the logits' type. */
+int dm_select_experts(const void* logits, int logits_are_bf16, int64_t stride, int64_t T, int E, int K, int sigmoid,
+                      const float* bias, int groups, int kept, int group_top, int renormalize, float scale, const void* mask,
+                      void* ids, int ids_are_int64, void* scores, int scores_are_bf16, void* stream);
+int dm_select_experts_bwd(const void* logits, int logits_are_bf16, int64_t stride, int64_t T, int E, int K, int sigmoid,
+                          int renormalize, float scale, const void* ids, int ids_are_int64, const void* grad_scores,
+                          int scores_are_bf16, void* grad_logits, void* stream);
+
+/* dm_few_tokens: the whole layer for up to DM_FEW_TOKENS_MAX tokens with bf16 weights, all experts local, in two launches.
+ * out[t] = sum_e c[t, e] W2[e] SwiGLU(W13[e] x[t]), c[t, e] = sum of the scores of token t's routes to expert e.  ids outside
+ * [0, E) go nowhere, other than -1 they are reported in `status`.  D % 32 == 0, F % 8 == 0, E <= 1024, K <= 32.  The workspace
+ * (dm_few_tokens_workspace_bytes, on the device of the launch; a negative DM_RC_* for an unsupported shape) is zeroed once before
+ * its first use and belongs to one call at a time. */
+#define DM_FEW_TOKENS_MAX 64
+int64_t dm_few_tokens_workspace_bytes(int64_t T, int64_t D, int64_t F, int E, int K);
+int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, const void* scores, int scores_are_bf16, const void* w13,
+                  const void* w2, void* out, int64_t T, int64_t D, int64_t F, int E, int K, int clamped, float alpha, float limit,
+                  void* workspace, int64_t workspace_bytes, int num_sms, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
