@@ -26,5 +26,5 @@ def run(x, ids, scores, w13, w2, state) -> torch.Tensor:
         x.data_ptr(), ids.data_ptr(), ids.dtype is torch.int64, scores.data_ptr(), scores.dtype is torch.bfloat16, w13.data_ptr(),
         w2.data_ptr(), out.data_ptr(), x.shape[0], cfg.hidden_dim, cfg.intermediate_dim, cfg.num_experts, cfg.top_k,
         cfg.activation == "swiglu_clamped", cfg.swiglu_alpha, cfg.swiglu_limit, ws.data_ptr(), ws.numel(), state.num_sms,
-        state.status.data_ptr(), nat.stream_ptr()), "dm_few_tokens", 2)
+        state.status.data_ptr(), nat.stream_ptr()), "dm_few_tokens")
     return out

@@ -157,9 +157,12 @@ class ContextState:
         self.clear_gather_flags()
 
     def clear_gather_flags(self) -> None:
-        """The fused dispatch finds its counters clear and leaves them clear.  Launches that ran at the same time (calls on one
-        context have to be ordered) may have left some of them behind, and later ones would take rows for gathered that are not."""
+        """The fused dispatch and the launch for few tokens find their counters clear and leave them clear.  Launches that ran at the
+        same time (calls on one context have to be ordered) may have left some of them behind, and later ones would take rows for
+        gathered that are not."""
         self.gather_flags.zero_()
+        if self.few_workspace is not None:
+            self.few_workspace.zero_()
 
     def select_slot(self, slot: int, num_layers: int) -> None:
         if self.num_slots == 0:

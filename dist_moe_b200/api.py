@@ -673,7 +673,7 @@ def routed_experts(x_TD: torch.Tensor | QuantizedRows, topk_expert_ids_TK: torch
 
 def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tensor, topk_scores_TK: torch.Tensor,
                               w13_weight: torch.Tensor, w2_weight: torch.Tensor, context: Context) -> torch.Tensor:
-    """:func:`routed_experts` for a decode step of up to 64 tokens, in two launches that stream the weights of the experts hit.
+    """:func:`routed_experts` for a decode step of up to 64 tokens, in one launch that streams the weights of the experts hit.
 
     ``out[t] = sum_e c[t, e] * W2[e] . SwiGLU(W13[e] . x[t])`` with ``c[t, e]`` the sum of token ``t``'s scores for expert ``e``.
     For BF16 contexts of one rank (all experts local), forward only: a call that autograd would record raises, as do block-scaled

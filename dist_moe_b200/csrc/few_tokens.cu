@@ -1,19 +1,20 @@
-// The whole routed-expert layer for up to 64 tokens, in two launches and without routing tables in memory.
+// The whole routed-expert layer for up to 64 tokens, in one launch and without routing tables in memory.
 //
 //   h[e, t] = c[t, e] * SwiGLU(W13[e] x[t]),   c[t, e] = sum of the scores of token t's routes to expert e   (bf16)
 //   out[t]  = sum_e W2[e] h[e, t]                                                                            (bf16)
-// Products and sums are in 32 bits; h is rounded once, with the score in it, so that the second launch sums over experts in its
+// Products and sums are in 32 bits; h is rounded once, with the score in it, so that the second product sums over experts in its
 // accumulators and has no weighted sum behind it.
 //
 // HBM bound: the weights of every expert that is hit stream through once (6 D F bytes each), all else is small.  So the weights never
-// wait: one warp of a block brings them into a ring in shared memory (an item by one tensor copy), another the rows of x or h that meet
-// them (512 bytes by one cp.async of the warp), and the second launch starts under the first (programmatic dependent launch) and has its first pieces of W2 on their way
-// before h is there.
+// wait: one warp of a block brings them into a ring in shared memory (an item by one tensor copy) and goes on from W13 to W2 at once,
+// another brings the rows of x or h that meet them (512 bytes by one cp.async of the warp) and alone waits for the other blocks where
+// h begins: by then 200 KB of W2 per SM are there.  All blocks are resident at once (cooperative launch), and that wait is bounded.
 //
 // A block works on strips of 32 weight rows (16 features of gate and up; 32 output columns); an item is 256 values of the inner
-// dimension of a strip, 16 KiB.  The items of all strips are dealt out evenly over the blocks, whatever the number of experts hit.  A
-// strip that is cut between blocks is summed by the one of them that finishes last, in the order of the blocks.  Of the eight warps
-// that multiply, four share an item's inner dimension and two its rows.
+// dimension of a strip, 16 KiB.  Where W13 has three strips or more for every block, blocks take them by tickets; else, and for W2, the
+// items of all strips are dealt out evenly over the blocks, whatever the number of experts hit.  A strip that is cut between blocks is
+// summed by the one of them that finishes last, in the order of the blocks.  The eight warps that multiply share an item's inner
+// dimension.
 //
 // With so few columns the products are mma.sync m16n8k16, weights as the 16-row operand, tokens as the 8 columns: both operands are
 // then read 16 bytes a lane along the inner dimension as they lie in shared memory, its order inside 32 values being the same for both
@@ -30,26 +31,35 @@ namespace dm {
 constexpr int kFewTokens = DM_FEW_TOKENS_MAX;
 constexpr int kFewExperts = 1024;
 constexpr int kFewTopK = 32;
-constexpr int kFewWarps = 8, kFewKWarps = 4;       // that multiply; side by side along the inner dimension
-constexpr int kFewThreads = 32 * (kFewWarps + 2);  // and one that loads weights, one that loads rows of x or h
-constexpr int kFewStep = 64 * kFewKWarps;          // values of the inner dimension per item
-constexpr int kFewRows = 32;                       // weight rows per strip
-constexpr int kFewLineBytes = kFewRows * 128;      // weights of an item: four lines of 64 values, 32 rows each
-constexpr int kFewWeightBytes = kFewKWarps * kFewLineBytes;
-constexpr int kFewRowPitch = kFewStep * 2 + 64;    // rows of x or h: eight of them 16 bytes a lane hit every bank once
+constexpr int kFewWarps = 8;                               // that multiply, side by side along the inner dimension
+constexpr int kFewThreads = 32 * (kFewWarps + 2);          // and one that loads weights, one that loads rows of x or h
+constexpr int kFewStep = 32 * kFewWarps;                  // values of the inner dimension per item
+constexpr int kFewLines = kFewStep / 64;                   // 128-byte lines of an item's rows
+constexpr int kFewRows = 32;                               // weight rows per strip
+constexpr int kFewLineBytes = kFewRows * 128;
+constexpr int kFewWeightBytes = kFewLines * kFewLineBytes;  // weights of an item
+constexpr int kFewRowPitch = kFewStep * 2 + 64;  // rows of x or h: eight of them, 16 bytes a lane, hit every bank once
 constexpr int kFewMaxDepth = 12;
+constexpr int kFewRedFloats = kFewWarps * kFewRows * 8;
+constexpr int kFewQueue = 4;                   // tickets on their way from the weights' warp to the others
+constexpr int kFewTicketStrips = 3;            // strips for every block from which on blocks draw tickets
+constexpr uint64_t kFewWaitNs = 2000000000ull;
 
+struct FewPhase {
+  CUtensorMap items;  // W13 (64 values, features, gate | up, lines, experts) or W2 (64 values, columns, lines, experts)
+  CUtensorMap tail;   // W2 with a last line of fewer than 64 values: (values, columns, experts)
+  float* partial;     // [blocks][2][kFewRows * 8 * tiles]
+  int32_t* arrived;   // [blocks][tiles][8 or 4 warps' outputs], clear between calls
+};
 struct FewParams {
-  CUtensorMap tm_w;     // items: W13 (64 values, features, gate | up, lines, experts) or W2 (64 values, columns, lines, experts)
-  CUtensorMap tm_tail;  // W2 with a last line of fewer than 64 values: (values, columns, experts)
+  FewPhase phase[2];  // W13, W2
   const __nv_bfloat16* x;
   const void* ids;
   const void* scores;
   int ids_are_int64, scores_are_bf16;
-  __nv_bfloat16* h;        // [pairs of expert and token][F]
-  float* partial;          // [blocks][2][kFewRows * 8 * tiles]
-  int32_t* arrived;        // per strip, clear between calls
+  __nv_bfloat16* h;  // [pairs of expert and token][F]
   __nv_bfloat16* out;
+  int32_t* meeting;  // blocks that have written their share of h; blocks that have seen it; tickets drawn.  Clear between calls
   int T, D, F, E, K;
   ActParams act;
   int* status;
@@ -58,7 +68,8 @@ struct FewParams {
 // Which experts are hit, by which tokens: built by every block.
 struct FewTables {
   uint64_t* tokens;  // [E] bit t: token t
-  float* share;      // [pairs] c[t, e]; W13 only
+  float* score;      // [T K]
+  float* share;      // [pairs] c[t, e]
   int16_t* expert;   // [active]
   int16_t* base;     // [active + 1] first pair
   int16_t* owner;    // [pairs] active expert
@@ -67,7 +78,8 @@ struct FewTables {
   __device__ __forceinline__ FewTables(uint8_t* at, int T, int E, int K) {
     const int active = T * K < E ? T * K : E;
     tokens = reinterpret_cast<uint64_t*>(at);
-    share = reinterpret_cast<float*>(tokens + E);
+    score = reinterpret_cast<float*>(tokens + E);
+    share = score + T * K;
     expert = reinterpret_cast<int16_t*>(share + T * K);
     base = expert + active;
     owner = base + active + 1;
@@ -75,7 +87,7 @@ struct FewTables {
     token = reinterpret_cast<uint8_t*>(id + T * K);
   }
   static __host__ __device__ constexpr int bytes(int T, int E, int K) {
-    return (8 * E + 9 * T * K + 4 * (T * K < E ? T * K : E) + 2 + 15) / 16 * 16;
+    return (8 * E + 13 * T * K + 4 * (T * K < E ? T * K : E) + 2 + 15) / 16 * 16;
   }
 };
 
@@ -93,6 +105,7 @@ __device__ __forceinline__ int few_tables(const FewParams& p, const FewTables& s
   for (int e = threadIdx.x; e < p.E; e += kFewThreads) s.tokens[e] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < p.T * p.K; i += kFewThreads) {
+    s.score[i] = p.scores_are_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.scores)[i]) : static_cast<const float*>(p.scores)[i];
     const int id = few_id(p, i);
     s.id[i] = static_cast<int16_t>(id);
     if (id >= 0)
@@ -176,8 +189,11 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 __device__ __forceinline__ void multipliers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory"); }
 // Row g of the instruction: neighbouring ones differ in the swizzle's third bit.
 __device__ __forceinline__ constexpr int few_row(int g) { return (g >> 1) | ((g & 1) << 2); }
-__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ int atom_add_acq_rel(int32_t* p, int v) {
+  int old;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
 
 // Where a block stands: strip, active expert, step of the inner dimension.  W13: strips of an expert follow one another; W2: the
 // experts of a strip do, and are summed.
@@ -210,155 +226,193 @@ struct FewCursor {
   }
 };
 
-// kTiles: tiles of eight columns that the accumulators hold; kRed: those that meet in shared memory at a time.
-template <bool kDown, int kTiles>
-__global__ void __launch_bounds__(kFewThreads, kTiles > 1 ? 1 : 2) few_tokens_kernel(const __grid_constant__ FewParams p, int ring_bytes) {
-  constexpr int kRed = kTiles > 2 ? 2 : kTiles;
-  constexpr int kWidth = 8 * kRed;
-  constexpr int kRedFloats = kFewKWarps * kFewRows * kWidth;
-  extern __shared__ __align__(1024) uint8_t few_smem_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kFewMaxDepth], empty[kFewMaxDepth];
-  __shared__ int s_found[2], s_last, abort_flag;
-  float* red = reinterpret_cast<float*>(ring + ring_bytes);  // [2][warps along the inner dimension][32 rows][kWidth]
-  const FewTables tab(ring + ring_bytes + 2 * kRedFloats * 4, p.T, p.E, p.K);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (!kDown) dependents_may_start();
-  if (warp == kFewWarps) {
-    if (lane < kFewMaxDepth) {
-      mbar_init(&full[lane], 1 + 32);  // the weights' warp and every lane of the rows' warp
-      mbar_init(&empty[lane], kFewWarps);
-    }
-    if (lane == 0) {
-      abort_flag = 0;
-    }
-    mbar_fence_init();
-    fence_proxy_async_smem();
+// What the warps of a block know of one of the two products.
+template <bool kDown>
+struct FewWork {
+  int inner, steps, strips, length, items;
+  FewSplit split;
+  FewCursor<kDown> begin;
+  bool tickets;  // strips are drawn one after another, the first one by the block's number; else the block has one run of items
+  __device__ __forceinline__ FewWork(const FewParams& p, int active)
+      : inner(kDown ? p.F : p.D),
+        steps((inner + kFewStep - 1) / kFewStep),
+        strips(kDown ? p.D / kFewRows : (p.F + 15) / 16),  // W13: of one expert
+        length(kDown ? active * steps : steps),            // items of a strip
+        split(kDown ? strips : static_cast<int64_t>(active) * strips, length, gridDim.x) {
+    const int64_t first = split.begin(blockIdx.x);
+    items = static_cast<int>(split.end(blockIdx.x) - first);
+    begin.set(0, 1, 1, 1);
+    tickets = !kDown && active * strips >= kFewTicketStrips * static_cast<int>(gridDim.x);
+    if (tickets)
+      draw(blockIdx.x, active);
+    else if (items > 0)
+      begin.set(first, strips, active, steps);
   }
-  int most;
-  const int active = few_tables(p, tab, s_found, !kDown && blockIdx.x == 0, most);
+  // The strip of a ticket; no items behind the last one.
+  __device__ __forceinline__ void draw(int ticket, int active) {
+    items = ticket < active * strips ? steps : 0;
+    if (items > 0) begin.set(static_cast<int64_t>(ticket) * steps, strips, active, steps);
+  }
+};
 
-  const int inner = kDown ? p.F : p.D;
-  const int steps = (inner + kFewStep - 1) / kFewStep;
-  const int strips = kDown ? p.D / kFewRows : (p.F + 15) / 16;  // W13: of one expert
-  const int length = kDown ? active * steps : steps;            // items of a strip
-  const FewSplit split(kDown ? strips : static_cast<int64_t>(active) * strips, length, gridDim.x);
-  const int64_t first = split.begin(blockIdx.x);
-  const int items = static_cast<int>(split.end(blockIdx.x) - first);
-  // A place of the ring: 16 KiB of weights, and as many rows of x or h as the expert with the most tokens has.
-  const int place_bytes = kFewWeightBytes + (most * kFewRowPitch + 1023) / 1024 * 1024;
-  const int depth = min(kFewMaxDepth, ring_bytes / place_bytes);
-  FewCursor<kDown> at;
-  at.set(0, 1, 1, 1);
-  if (items > 0) at.set(first, strips, active, steps);
+struct FewQueue {
+  uint64_t* full;
+  uint64_t* empty;
+  int* ticket;
+  int n;  // tickets seen
+  __device__ __forceinline__ int place() const { return n & (kFewQueue - 1); }
+  __device__ __forceinline__ uint32_t round() const { return (n / kFewQueue) & 1; }
+  // The next ticket, for a whole warp; -1 if it did not come in time.
+  __device__ __forceinline__ int next(int* abort_flag, int lane) {
+    if (!warp_mbar_wait(&full[place()], round(), abort_flag)) return -1;
+    const int got = ticket[place()];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[place()]);
+    ++n;
+    return got;
+  }
+};
 
-  if (warp == kFewWarps) {
-    // ======================= weights =======================
-    const bool elected = elect_one();
-    int place = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int i = 0; i < items; ++i) {
-      ok = warp_mbar_wait(&empty[place], phase ^ 1u, &abort_flag);
-      if (!ok) break;
-      uint8_t* to = ring + place * place_bytes;
+struct FewRing {
+  uint8_t* base;
+  uint64_t* full;
+  uint64_t* empty;
+  int* abort_flag;
+  int place_bytes, depth;
+  int place;
+  uint32_t round;  // parity of the ring's round
+  __device__ __forceinline__ void next() {
+    if (++place == depth) {
+      place = 0;
+      round ^= 1u;
+    }
+  }
+};
+
+// The weights' warp, all lanes.  Returns whether every place became free in time.
+template <bool kDown>
+__device__ __forceinline__ bool few_load_weights(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, bool elected,
+                                                 int lane) {
+  FewWork<kDown> work(p, active);
+  const FewPhase& phase = p.phase[kDown];
+  while (true) {
+    int next = 0;
+    if (work.tickets && work.items > 0 && lane == 0) next = gridDim.x + atomicAdd(p.meeting + 2, 1);  // here by the end of this strip
+    FewCursor<kDown> at = work.begin;
+    for (int i = 0; i < work.items; ++i) {
+      if (!warp_mbar_wait(&ring.empty[ring.place], ring.round ^ 1u, ring.abort_flag)) return false;
+      uint8_t* to = ring.base + ring.place * ring.place_bytes;
+      uint64_t* full = &ring.full[ring.place];
       const int e = uniform(static_cast<int>(tab.expert[at.a])), strip = uniform(at.strip), c = uniform(at.c);
-      const int lines = min(kFewKWarps, (inner - c * kFewStep + 63) / 64);
       if (elected) {
-        if (kDown && (c + 1) * kFewStep > inner && (inner & 63) != 0) {
-          mbar_arrive_expect_tx(&full[place], lines * kFewLineBytes);
+        if (kDown && (c + 1) * kFewStep > work.inner && (work.inner & 63) != 0) {
+          const int lines = min(kFewLines, (work.inner - c * kFewStep + 63) / 64);
+          mbar_arrive_expect_tx(full, lines * kFewLineBytes);
           for (int l = 0; l < lines; ++l)
-            tma_load_3d(to + l * kFewLineBytes, &p.tm_tail, c * kFewStep + 64 * l, strip * kFewRows, e, &full[place]);
+            tma_load_3d(to + l * kFewLineBytes, &phase.tail, c * kFewStep + 64 * l, strip * kFewRows, e, full);
         } else {
-          mbar_arrive_expect_tx(&full[place], kFewWeightBytes);
+          mbar_arrive_expect_tx(full, kFewWeightBytes);
           if (kDown)
-            tma_load_4d(to, &p.tm_w, 0, strip * kFewRows, c * kFewKWarps, e, &full[place]);
+            tma_load_4d(to, &phase.items, 0, strip * kFewRows, c * kFewLines, e, full);
           else
-            tma_load_5d(to, &p.tm_w, 0, strip * 16, 0, c * kFewKWarps, e, &full[place]);
+            tma_load_5d(to, &phase.items, 0, strip * 16, 0, c * kFewLines, e, full);
         }
       }
       __syncwarp();
-      at.next(strips, active, steps);
-      if (++place == depth) {
-        place = 0;
-        phase ^= 1u;
-      }
+      at.next(work.strips, active, work.steps);
+      ring.next();
     }
-    if (lane == 0) {  // what is on its way has to land before the block gives its shared memory back
-      if (!ok) set_status(p.status, kPipelineTimeout, 6, blockIdx.x);
-      settle_ring(full, depth, ring_stop(place, phase), globaltimer_ns() + (ok ? 2000000000ull : kSettleNs));
+    if (!work.tickets || work.items == 0) return true;
+    next = uniform(next);
+    if (!warp_mbar_wait(&queue.empty[queue.place()], queue.round() ^ 1u, ring.abort_flag)) return false;
+    if (lane == 0) {
+      queue.ticket[queue.place()] = next;
+      mbar_arrive(&queue.full[queue.place()]);
     }
-    return;
+    __syncwarp();
+    ++queue.n;
+    work.draw(next, active);
   }
-  if (warp == kFewWarps + 1) {
-    // ======================= rows of x or h =======================
-    if (kDown) wait_for_launch_before();  // h is there from here on
-    const uint32_t own = smem_u32(ring) + kFewWeightBytes + lane * 16;
-    int place = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int i = 0; i < items; ++i) {
-      ok = warp_mbar_wait(&empty[place], phase ^ 1u, &abort_flag);
-      if (!ok) break;
+}
+
+// The rows' warp, all lanes: the expert's rows next to one another.
+template <bool kDown>
+__device__ __forceinline__ bool few_load_rows(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, int lane) {
+  FewWork<kDown> work(p, active);
+  const uint32_t own = smem_u32(ring.base) + kFewWeightBytes + lane * 16;
+  while (true) {
+    FewCursor<kDown> at = work.begin;
+    for (int i = 0; i < work.items; ++i) {
+      if (!warp_mbar_wait(&ring.empty[ring.place], ring.round ^ 1u, ring.abort_flag)) return false;
       const int k = at.c * kFewStep + lane * 8;
-      const bool in = k < inner;
+      const bool in = k < work.inner;
       const int base = tab.base[at.a], count = tab.base[at.a + 1] - base;
-      const __nv_bfloat16* source = (kDown ? p.h + static_cast<int64_t>(base) * inner : p.x) + (in ? k : 0);
+      const __nv_bfloat16* source = (kDown ? p.h + static_cast<int64_t>(base) * work.inner : p.x) + (in ? k : 0);
+      const uint32_t to = own + ring.place * ring.place_bytes;
 #pragma unroll 4
       for (int j = 0; j < count; ++j)
-        cp_async16(own + place * place_bytes + j * kFewRowPitch, source + static_cast<int64_t>(kDown ? j : tab.token[base + j]) * inner, in);
-      cp_async_arrive(&full[place]);
-      at.next(strips, active, steps);
-      if (++place == depth) {
-        place = 0;
-        phase ^= 1u;
-      }
+        cp_async16(to + j * kFewRowPitch, source + static_cast<int64_t>(kDown ? j : tab.token[base + j]) * work.inner, in);
+      cp_async_arrive(&ring.full[ring.place]);
+      at.next(work.strips, active, work.steps);
+      ring.next();
     }
-    if (!ok && lane == 0) set_status(p.status, kPipelineTimeout, 8, blockIdx.x);
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    return;
+    if (!work.tickets || work.items == 0) return true;
+    const int next = queue.next(ring.abort_flag, lane);
+    if (next < 0) return false;
+    work.draw(next, active);
   }
+}
 
-  // ======================= products =======================
-  if (kDown) {
-    wait_for_launch_before();
-    if (active == 0) {
-      const int64_t n = static_cast<int64_t>(p.T) * p.D;
-      for (int64_t i = blockIdx.x * static_cast<int64_t>(32 * kFewWarps) + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 32 * kFewWarps)
-        p.out[i] = __float2bfloat16_rn(0.f);
-      return;
-    }
-  } else {
-    for (int i = threadIdx.x; i < tab.base[active]; i += 32 * kFewWarps) {
-      const int t = tab.token[i], e = tab.expert[tab.owner[i]];
-      float share = 0.f;
-      for (int k = 0; k < p.K; ++k)
-        if (tab.id[t * p.K + k] == e)
-          share += p.scores_are_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.scores)[t * p.K + k])
-                                     : static_cast<const float*>(p.scores)[t * p.K + k];
-      tab.share[i] = share;
-    }
-  }
-  const int g = lane >> 2, quad = lane & 3, kw = warp & (kFewKWarps - 1), half = warp / kFewKWarps;
+__device__ __forceinline__ bool try_wait_addr(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void arrive_addr(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A wait that ran out is recorded; the block goes on without its data, so that its warps still meet.
+__device__ __noinline__ void few_wait_on(uint64_t* bar, uint32_t parity, int* abort_flag, int* status) {
+  if (!mbar_wait(bar, parity, abort_flag)) set_status(status, kPipelineTimeout, 7, blockIdx.x);
+}
+
+// The warps that multiply.  kTiles: tiles of eight columns that the accumulators hold.  `turn`: which warps look after the next sums.
+template <bool kDown, int kTiles>
+__device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, float* red,
+                                             int* s_next, uint32_t zeros, int& turn) {
+  FewWork<kDown> work(p, active);
+  const FewPhase& phase = p.phase[kDown];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, quad = lane & 3;
   const int rho = few_row(g);
-  // W13: rows 0 to 15 of a tile are gate features, 16 to 31 the same features of up
-  const int r0 = kDown ? 16 * half + rho : 8 * half + rho, r1 = kDown ? r0 + 8 : r0 + 16;
-  const uint32_t line = smem_u32(ring) + kw * kFewLineBytes;
-  const uint32_t at_w = line + r0 * 128 + ((quad ^ rho) << 4);  // the other 32 values of the line: 64 bytes on or back
-  const uint32_t at_b = smem_u32(ring) + kFewWeightBytes + kw * 128 + quad * 16;
-  const int up = (r1 - r0) * 128;
-
-  float acc[kTiles][4];
+  // Rows of the lane: rho, rho + up and both with `half` more.  W13: rows 0 to 15 of an item are gate features, 16 to 31 those of up.
+  constexpr int half = kDown ? 16 : 8, up = kDown ? 8 : 16;
+  const uint32_t at_w = smem_u32(ring.base) + (warp >> 1) * kFewLineBytes + rho * 128 + ((((warp & 1) * 4 + quad) ^ rho) << 4);
+  const uint32_t at_b = smem_u32(ring.base) + kFewWeightBytes + warp * 64 + quad * 16;
+  const uint32_t none = zeros + warp * 64 + quad * 16;
+  const uint32_t full0 = smem_u32(ring.full), empty0 = smem_u32(ring.empty);
+  int place = ring.place;
+  uint32_t round = ring.round, here = place * ring.place_bytes;
+  float acc[2][kTiles][4];
   auto clear = [&] {
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.f;
   };
-  // Columns: W13 the expert's tokens; W2 all tokens, those that are not the expert's being zero.
+  // Columns.  W13: the expert's tokens; those beyond the last one repeat it and are not kept.  W2: all tokens, those that are not the
+  // expert's being zero.
   int tiles = 0;
-  int from[kTiles];  // offset of the column's row in a place; W2: -1 for none
-  uint32_t hit = 0;  // W2: tiles that any token of the expert is in
+  int from[kTiles];  // offset of the column's row in a place, W2: -1 for none
+  uint32_t hit = 0;  // tiles that any token of the expert is in
   auto columns = [&](int a) {
     if (kDown) {
       const uint64_t tokens = tab.tokens[tab.expert[a]];
@@ -374,123 +428,229 @@ __global__ void __launch_bounds__(kFewThreads, kTiles > 1 ? 1 : 2) few_tokens_ke
       const int count = tab.base[a + 1] - tab.base[a];
       tiles = (count + 7) >> 3;
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) from[n] = 8 * n + g < count ? (8 * n + g) * kFewRowPitch : -1;
+      for (int n = 0; n < kTiles; ++n) from[n] = min(8 * n + g, count - 1) * kFewRowPitch;
       hit = (1u << tiles) - 1;
     }
   };
-  clear();
-  if (items > 0) columns(at.a);
-
-  int place = 0, flip = 0;
-  uint32_t phase = 0;
-  int began = at.c + (kDown ? at.a * steps : 0);  // first item of the strip that this block has
-  for (int item = 0; item < items; ++item) {
-    // A wait that ran out is recorded; the block goes on without its data, so that its warps still meet.
-    if (!warp_mbar_wait(&full[place], phase, &abort_flag) && lane == 0) set_status(p.status, kPipelineTimeout, 7, blockIdx.x);
-    const uint32_t here = place * place_bytes;
-    const int k = at.c * kFewStep + kw * 64;
-    if (k < inner) {  // beyond the last value weights and rows are zero
+  // `n_items` items in a row; `first_alone`: no tile but the first is hit
+  auto run = [&](int c, int n_items, auto first_alone) {
+    int k = c * kFewStep + warp * 32;
+#pragma unroll 1
+    for (int i = 0; i < n_items; ++i, k += kFewStep) {
+      if (!try_wait_addr(full0 + 8 * place, round)) few_wait_on(ring.full + place, round, ring.abort_flag, p.status);
+      if (k < work.inner) {  // beyond the last value weights and rows are zero
+        const uint32_t aw = at_w + here;
+        const uint4 lo0 = lds16(aw), hi0 = lds16(aw + up * 128), lo1 = lds16(aw + half * 128), hi1 = lds16(aw + (half + up) * 128);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t aw = (at_w + here) ^ (h << 6);
-        const uint4 lo = lds16(aw), hi = lds16(aw + up);
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          if (((hit >> n) & 1) == 0) continue;
-          uint4 b = make_uint4(0, 0, 0, 0);
-          if (from[n] >= 0) b = lds16(at_b + here + h * 64 + from[n]);
-          mma_16x8x16(acc[n], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
-          mma_16x8x16(acc[n], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+        for (int n = 0; n < (decltype(first_alone)::value ? 1 : kTiles); ++n) {
+          if (!decltype(first_alone)::value && ((hit >> n) & 1) == 0) continue;
+          const uint4 b = lds16(kDown && from[n] < 0 ? none : at_b + here + from[n]);
+          mma_16x8x16(acc[0][n], lo0.x, hi0.x, lo0.y, hi0.y, b.x, b.y);
+          mma_16x8x16(acc[1][n], lo1.x, hi1.x, lo1.y, hi1.y, b.x, b.y);
+          mma_16x8x16(acc[0][n], lo0.z, hi0.z, lo0.w, hi0.w, b.z, b.w);
+          mma_16x8x16(acc[1][n], lo1.z, hi1.z, lo1.w, hi1.w, b.z, b.w);
         }
       }
+      __syncwarp();
+      if (lane == 0) arrive_addr(empty0 + 8 * place);
+      ++place;
+      here += ring.place_bytes;
+      if (place == ring.depth) {
+        place = 0;
+        here = 0;
+        round ^= 1u;
+      }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[place]);
-    if (++place == depth) {
-      place = 0;
-      phase ^= 1u;
-    }
+  };
+  clear();
+  FewCursor<kDown> at = work.begin;
+  int strip_no = 0;  // two places for the next ticket: a warp may still read one while the next strip's is written
+  bool whole = at.c == 0 && (!kDown || at.a == 0);  // the strip from its first item on
+  for (int left = work.items; left > 0;) {
+    columns(at.a);
+    const int n_items = min(left, work.steps - at.c);
+    if (kTiles == 1 || hit == 1)
+      run(at.c, n_items, std::true_type{});
+    else
+      run(at.c, n_items, std::false_type{});
+    left -= n_items;
     const FewCursor<kDown> done = at;
-    at.next(strips, active, steps);
+    at.c += n_items - 1;
+    at.next(work.strips, active, work.steps);
     const bool strip_end = kDown ? at.strip != done.strip : at.c == 0;
-    if (!strip_end && item + 1 < items) {
-      if (kDown && at.a != done.a) columns(at.a);
-      continue;
-    }
-    // ---- sum over the warps, kRed tiles at a time, in two buffers in turn: one barrier each --------------------------
+    if (!strip_end && left > 0) continue;
+    // ---- sum over the warps, a tile at a time, in two buffers in turn: one barrier each.  The warps take turns at what follows it; the
+    // others go on with the next strip. ------------------------------------------------------------------------------
+    whole = whole && strip_end;
     const int base = tab.base[done.a], count = kDown ? p.T : tab.base[done.a + 1] - base;
-    const bool whole = strip_end && began == 0;
-    const int64_t q = kDown ? done.strip : static_cast<int64_t>(done.a) * strips + done.strip;  // strip of the launch
-    auto part = [&](int block) { return p.partial + split.place(block, q) * (kFewRows * 8 * kTiles); };
-    // `value(r, col)`: sum of weight row r of the strip and column col
-    auto finish = [&](int col0, int cols, auto&& value) {
-      if (kDown) {
-        for (int i = threadIdx.x; i < kFewRows * cols; i += 32 * kFewWarps) {
-          const int r = i & (kFewRows - 1), col = col0 + i / kFewRows;
-          p.out[static_cast<int64_t>(col) * p.D + done.strip * kFewRows + r] = __float2bfloat16_rn(value(r, col));
+    constexpr int kOut = kDown ? kFewRows : 16;  // outputs of a column
+    int drawn = 0;
+#pragma unroll 1
+    for (int n = 0; n < tiles; ++n) {
+      float* buf = red + (turn & 1) * kFewRedFloats;
+      float* to = buf + (warp * kFewRows + rho) * 8 + 2 * quad;
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m)
+        if (m == n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            *reinterpret_cast<float2*>(to + i * half * 8) = make_float2(acc[i][m][0], acc[i][m][1]);
+            *reinterpret_cast<float2*>(to + (i * half + up) * 8) = make_float2(acc[i][m][2], acc[i][m][3]);
+          }
+      if (work.tickets && n == 0 && warp == 0) {  // one warp decides for all: they stay together where the ticket does not come
+        const int next = queue.next(ring.abort_flag, lane);
+        if (lane == 0) s_next[strip_no & 1] = next < 0 ? 0x7fffffff : next;
+      }
+      multipliers_meet();
+      if (work.tickets && n == 0) drawn = s_next[strip_no & 1];
+      const int cols = min(count - 8 * n, 8);
+      const int slot = (warp + turn * (kOut * 8 / 32)) & (kFewWarps - 1);  // of 32 outputs
+      ++turn;
+      if (slot * 32 >= kOut * cols) continue;
+      const int o = slot * 32 + lane, r = o & (kOut - 1), col = 8 * n + o / kOut;
+      const bool in = o < kOut * cols;
+      float v = 0.f, u = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) {
+        v += buf[(w * kFewRows + r) * 8 + (o / kOut)];
+        if (!kDown) u += buf[(w * kFewRows + 16 + r) * 8 + (o / kOut)];
+      }
+      bool mine = true;  // to finish these outputs
+      if (!whole) {
+        const int64_t q = kDown ? done.strip : static_cast<int64_t>(done.a) * work.strips + done.strip;  // strip of the product
+        const int first = work.split.first_block(q), last = work.split.last_block(q);
+        const int at_out = (8 * n * kOut + o) * (kDown ? 1 : 2);
+        auto part = [&](int block) { return phase.partial + work.split.place(block, q) * (kFewRows * 8 * kTiles) + at_out; };
+        if (kDown)
+          __stcg(part(blockIdx.x), v);
+        else
+          __stcg(reinterpret_cast<float2*>(part(blockIdx.x)), make_float2(v, u));
+        // every block's warp with these outputs arrives; the last one finds all parts there
+        int32_t* arrived = phase.arrived + (first * kTiles + n) * (kOut * 8 / 32) + slot;
+        __syncwarp();
+        int before = 0;
+        if (lane == 0) {
+          before = atom_add_acq_rel(arrived, 1);
+          if (before == last - first) *arrived = 0;  // clear for the next call
         }
-      } else {
-        for (int i = threadIdx.x; i < 16 * cols; i += 32 * kFewWarps) {
-          const int f = done.strip * 16 + (i & 15), col = col0 + (i >> 4);
-          if (f >= p.F) continue;
-          const float gate[1] = {value(i & 15, col)}, up1[1] = {value(16 + (i & 15), col)};
+        mine = __shfl_sync(0xffffffffu, before, 0) == last - first;
+        if (mine) {
+          v = u = 0.f;
+          for (int block = first; block <= last; ++block) {
+            if (kDown) {
+              v += __ldcg(part(block));
+            } else {
+              const float2 vu = __ldcg(reinterpret_cast<const float2*>(part(block)));
+              v += vu.x;
+              u += vu.y;
+            }
+          }
+        }
+      }
+      if (mine && in) {
+        if (kDown) {
+          p.out[static_cast<int64_t>(col) * p.D + done.strip * kFewRows + r] = __float2bfloat16_rn(v);
+        } else if (done.strip * 16 + r < p.F) {
+          const float gate[1] = {v}, up1[1] = {u};
           float z[1];
           swiglu_f32(gate, up1, z, p.act);
-          p.h[static_cast<int64_t>(base + col) * p.F + f] = __float2bfloat16_rn(tab.share[base + col] * z[0]);
+          p.h[static_cast<int64_t>(base + col) * p.F + done.strip * 16 + r] = __float2bfloat16_rn(tab.share[base + col] * z[0]);
         }
-      }
-    };
-#pragma unroll
-    for (int n0 = 0; n0 < kTiles; n0 += kRed) {
-      if (n0 >= tiles) break;
-      float* buf = red + flip * kRedFloats;
-      flip ^= 1;
-#pragma unroll
-      for (int n = 0; n < kRed; ++n) {
-        float* to = buf + (kw * kFewRows + r0) * kWidth + 8 * n + 2 * quad;
-        *reinterpret_cast<float2*>(to) = make_float2(acc[n0 + n][0], acc[n0 + n][1]);
-        *reinterpret_cast<float2*>(to + (r1 - r0) * kWidth) = make_float2(acc[n0 + n][2], acc[n0 + n][3]);
-      }
-      multipliers_meet();
-      const int col0 = 8 * n0, cols = min(count - col0, kWidth);
-      auto sum_of = [&](int r, int col) {
-        float v = 0.f;
-#pragma unroll
-        for (int w4 = 0; w4 < kFewKWarps; ++w4) v += buf[(w4 * kFewRows + r) * kWidth + col - col0];
-        return v;
-      };
-      if (whole) {
-        finish(col0, cols, sum_of);
-      } else {
-        float* mine = part(blockIdx.x);
-        for (int i = threadIdx.x; i < kFewRows * cols; i += 32 * kFewWarps) {
-          const int r = i & (kFewRows - 1), col = col0 + i / kFewRows;
-          __stcg(mine + col * kFewRows + r, sum_of(r, col));
-        }
-      }
-    }
-    if (!whole) {
-      __threadfence();
-      multipliers_meet();
-      if (threadIdx.x == 0) {
-        const int before = atomicAdd(p.arrived + q, 1);
-        s_last = before == split.last_block(q) - split.first_block(q);
-        if (s_last) p.arrived[q] = 0;  // clear for the next call
-        __threadfence();
-      }
-      multipliers_meet();
-      if (s_last) {
-        const int begin = split.first_block(q), last = split.last_block(q);
-        finish(0, count, [&](int r, int col) {
-          float v = 0.f;
-          for (int block = begin; block <= last; ++block) v += __ldcg(part(block) + col * kFewRows + r);
-          return v;
-        });
       }
     }
     clear();
-    began = 0;
-    if (item + 1 < items) columns(at.a);
+    whole = true;
+    if (work.tickets) {
+      ++strip_no;
+      work.draw(drawn, active);
+      at = work.begin;
+      left = work.items;
+    }
+  }
+  ring.place = place;
+  ring.round = round;
+}
+
+template <int kTiles>
+__global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid_constant__ FewParams p, int ring_bytes) {
+  extern __shared__ __align__(1024) uint8_t few_smem_raw[];
+  uint8_t* smem = few_smem_raw + (-smem_u32(few_smem_raw) & 1023u);  // an offset: what lies there stays known as shared memory
+  __shared__ uint64_t full[kFewMaxDepth], empty[kFewMaxDepth], queue_full[kFewQueue], queue_empty[kFewQueue];
+  __shared__ int s_found[2], s_ticket[kFewQueue], s_next[2], abort_flag;
+  __shared__ __align__(16) uint8_t zeros[kFewStep * 2];  // a row for the columns that an expert has none for
+  float* red = reinterpret_cast<float*>(smem + ring_bytes);  // [2][warps along the inner dimension][32 rows][8]
+  const FewTables tab(smem + ring_bytes + 2 * kFewRedFloats * 4, p.T, p.E, p.K);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == kFewWarps) {
+    if (lane < kFewMaxDepth) {
+      mbar_init(&full[lane], 1 + 32);  // the weights' warp and every lane of the rows' warp
+      mbar_init(&empty[lane], kFewWarps);
+    }
+    if (lane < kFewQueue) {
+      mbar_init(&queue_full[lane], 1);
+      mbar_init(&queue_empty[lane], 2);  // the rows' warp and one for those that multiply
+    }
+    if (lane == 0) {
+      abort_flag = 0;
+      tma_prefetch_desc(&p.phase[0].items);
+      tma_prefetch_desc(&p.phase[1].items);
+    }
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  if (threadIdx.x < sizeof(zeros) / 4) reinterpret_cast<uint32_t*>(zeros)[threadIdx.x] = 0;
+  int most;
+  const int active = few_tables(p, tab, s_found, blockIdx.x == 0, most);
+  if (active == 0) {  // nothing is routed anywhere: all blocks see it
+    const int64_t n = static_cast<int64_t>(p.T) * p.D;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kFewThreads) + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * kFewThreads)
+      p.out[i] = __float2bfloat16_rn(0.f);
+    return;
+  }
+  // A place of the ring: 16 KiB of weights, and as many rows of x or h as the expert with the most tokens has.
+  FewRing ring{smem, full, empty, &abort_flag, kFewWeightBytes + (most * kFewRowPitch + 1023) / 1024 * 1024, 0, 0, 0};
+  ring.depth = min(kFewMaxDepth, ring_bytes / ring.place_bytes);
+  FewQueue queue{queue_full, queue_empty, s_ticket, 0};
+
+  if (warp == kFewWarps) {
+    const bool elected = elect_one();
+    const bool ok = few_load_weights<false>(p, tab, ring, queue, active, elected, lane) &&
+                    few_load_weights<true>(p, tab, ring, queue, active, elected, lane);
+    if (lane == 0) {  // what is on its way has to land before the block gives its shared memory back
+      if (!ok) set_status(p.status, kPipelineTimeout, 6, blockIdx.x);
+      settle_ring(full, ring.depth, ring_stop(ring.place, ring.round), globaltimer_ns() + (ok ? kFewWaitNs : kSettleNs));
+    }
+  } else if (warp == kFewWarps + 1) {
+    bool ok = few_load_rows<false>(p, tab, ring, queue, active, lane);
+    if (ok) {  // until h is there
+      const uint64_t t0 = globaltimer_ns();
+      uint32_t spins = 0;
+      while (ok && ld_acquire_gpu(p.meeting) < static_cast<int>(gridDim.x))
+        if ((++spins & 0xff) == 0 && (*const_cast<volatile int*>(&abort_flag) != 0 || globaltimer_ns() - t0 > kFewWaitNs)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      // the last one to leave clears them for the next call: every block has drawn its last ticket
+      if (ok && lane == 0 && atom_add_acq_rel(p.meeting + 1, 1) == static_cast<int>(gridDim.x) - 1) p.meeting[0] = p.meeting[1] = p.meeting[2] = 0;
+      __syncwarp();
+    }
+    ok = ok && few_load_rows<true>(p, tab, ring, queue, active, lane);
+    if (!ok && lane == 0) {
+      *const_cast<volatile int*>(&abort_flag) = 1;
+      set_status(p.status, kPipelineTimeout, 8, blockIdx.x);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    for (int i = threadIdx.x; i < tab.base[active]; i += 32 * kFewWarps) {  // read behind the first strip's barrier
+      const int t = tab.token[i], e = tab.expert[tab.owner[i]];
+      float share = 0.f;
+      for (int k = 0; k < p.K; ++k)
+        if (tab.id[t * p.K + k] == e) share += tab.score[t * p.K + k];
+      tab.share[i] = share;
+    }
+    int turn = 0;
+    few_multiply<false, kTiles>(p, tab, ring, queue, active, red, s_next, smem_u32(zeros), turn);
+    multipliers_meet();  // the block's share of h is written
+    if (threadIdx.x == 0) red_release_gpu_add(p.meeting, 1);
+    few_multiply<true, kTiles>(p, tab, ring, queue, active, red, s_next, smem_u32(zeros), turn);
   }
 }
 
@@ -503,7 +663,7 @@ static int few_encode(CUtensorMap* tm, const void* w, int64_t D, int64_t F, int6
   const cuuint64_t dims13[5] = {64, f, 2, d / 64, e}, strides13[4] = {2 * d, 2 * f * d, 128, 4 * f * d};
   const cuuint64_t dims2[4] = {64, d, f / 64, e}, strides2[3] = {2 * f, 128, 2 * f * d};
   const cuuint64_t dims_tail[3] = {f, d, e}, strides_tail[2] = {2 * f, 2 * f * d};
-  const cuuint32_t box13[5] = {64, 16, 2, kFewKWarps, 1}, box2[4] = {64, kFewRows, kFewKWarps, 1}, box_tail[3] = {64, kFewRows, 1};
+  const cuuint32_t box13[5] = {64, 16, 2, kFewLines, 1}, box2[4] = {64, kFewRows, kFewLines, 1}, box_tail[3] = {64, kFewRows, 1};
   const cuuint32_t step[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, tail ? 3 : down ? 4 : 5, const_cast<void*>(w),
                          tail ? dims_tail : down ? dims2 : dims13, tail ? strides_tail : down ? strides2 : strides13,
@@ -513,16 +673,17 @@ static int few_encode(CUtensorMap* tm, const void* w, int64_t D, int64_t F, int6
 }
 
 struct FewLayout {
-  int64_t arrived13, arrived2, partial13, partial2, h, total;
+  int64_t meeting, arrived13, arrived2, partial13, partial2, h, total;
 };
-static FewLayout few_layout(int64_t T, int64_t D, int64_t F, int64_t E, int64_t K) {
-  const int64_t active = T * K < E ? T * K : E;
+static FewLayout few_layout(int64_t T, int64_t F, int64_t K) {
   auto a128 = [](int64_t v) { return (v + 127) / 128 * 128; };
-  const int64_t partial = a128(static_cast<int64_t>(sm_count()) * 2 * kFewRows * kFewTokens * 4);
+  const int64_t blocks = sm_count(), tiles = T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8;
+  const int64_t partial = a128(blocks * 2 * kFewRows * 8 * tiles * 4), arrived = a128(blocks * tiles * 8 * 4);
   FewLayout l;
-  l.arrived13 = 0;
-  l.arrived2 = l.arrived13 + a128(active * ((F + 15) / 16) * 4);
-  l.partial13 = l.arrived2 + a128(D / kFewRows * 4);
+  l.meeting = 0;
+  l.arrived13 = 128;
+  l.arrived2 = l.arrived13 + arrived;
+  l.partial13 = l.arrived2 + arrived;
   l.partial2 = l.partial13 + partial;
   l.h = l.partial2 + partial;
   l.total = l.h + a128(T * K * F * 2);
@@ -541,7 +702,7 @@ using namespace dm;
 
 extern "C" int64_t dm_few_tokens_workspace_bytes(int64_t T, int64_t D, int64_t F, int E, int K) {
   const int rc = few_shape(T, D, F, E, K);
-  return rc != kRcOk ? rc : few_layout(T, D, F, E, K).total;
+  return rc != kRcOk ? rc : few_layout(T, F, K).total;
 }
 
 extern "C" int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, const void* scores, int scores_are_bf16,
@@ -553,7 +714,7 @@ extern "C" int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, 
   if (rc != kRcOk) return rc;
   for (const void* v : {x, w13, w2, static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(v) % 16 != 0) return kRcBadArg;
-  const FewLayout l = few_layout(T, D, F, E, K);
+  const FewLayout l = few_layout(T, F, K);
   if (workspace_bytes < l.total) return kRcBadArg;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   FewParams p{};
@@ -564,17 +725,21 @@ extern "C" int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, 
   p.scores_are_bf16 = scores_are_bf16;
   p.h = reinterpret_cast<__nv_bfloat16*>(ws + l.h);
   p.out = static_cast<__nv_bfloat16*>(out);
+  p.meeting = reinterpret_cast<int32_t*>(ws + l.meeting);
   p.T = static_cast<int>(T), p.D = static_cast<int>(D), p.F = static_cast<int>(F), p.E = E, p.K = K;
   p.act = ActParams{clamped, alpha, limit};
   p.status = status;
-  const unsigned grid = static_cast<unsigned>(persistent_grid(num_sms));
-  auto run = [&](auto down_tag, auto tiles_tag) {
-    constexpr bool down = decltype(down_tag)::value;
-    constexpr int tiles = decltype(tiles_tag)::value;
-    constexpr auto kernel = few_tokens_kernel<down, tiles>;
-    constexpr int red = 2 * kFewKWarps * kFewRows * 8 * (tiles > 2 ? 2 : tiles) * 4;
-    // Up to eight tokens a block leaves room for one of the other launch on its SM.
-    constexpr int most = tiles > 1 ? 226 * 1024 : 112 * 1024;
+  p.phase[0].partial = reinterpret_cast<float*>(ws + l.partial13);
+  p.phase[0].arrived = reinterpret_cast<int32_t*>(ws + l.arrived13);
+  p.phase[1].partial = reinterpret_cast<float*>(ws + l.partial2);
+  p.phase[1].arrived = reinterpret_cast<int32_t*>(ws + l.arrived2);
+  rc = few_encode(&p.phase[0].items, w13, D, F, E, false, false);
+  if (rc == kRcOk && F >= 64) rc = few_encode(&p.phase[1].items, w2, D, F, E, true, false);
+  if (rc == kRcOk && F % 64 != 0) rc = few_encode(&p.phase[1].tail, w2, D, F, E, true, true);
+  if (rc != kRcOk) return rc;
+  auto run = [&](auto tiles_tag) {
+    constexpr auto kernel = few_tokens_kernel<decltype(tiles_tag)::value>;
+    constexpr int most = 226 * 1024, red = 2 * kFewRedFloats * 4;
     const int tables = FewTables::bytes(p.T, p.E, p.K);
     const int ring = (most - 1024 - red - tables) / 1024 * 1024;
     static PerDeviceOnce attr_set;
@@ -582,31 +747,21 @@ extern "C" int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, 
       return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     });
     if (arc != 0) return arc;
-    FewParams q = p;
-    int erc = !down || F >= 64 ? few_encode(&q.tm_w, down ? w2 : w13, D, F, E, down, false) : kRcOk;
-    if (erc == kRcOk && down && F % 64 != 0) erc = few_encode(&q.tm_tail, w2, D, F, E, true, true);
-    if (erc != kRcOk) return erc;
-    q.partial = reinterpret_cast<float*>(ws + (down ? l.partial2 : l.partial13));
-    q.arrived = reinterpret_cast<int32_t*>(ws + (down ? l.arrived2 : l.arrived13));
     cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    attr.id = cudaLaunchAttributeCooperative;  // the blocks meet once: all of them are resident
+    attr.val.cooperative = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid);
+    config.gridDim = dim3(static_cast<unsigned>(persistent_grid(num_sms)));
     config.blockDim = dim3(kFewThreads);
     config.dynamicSmemBytes = 1024 + ring + red + tables;
     config.stream = static_cast<cudaStream_t>(stream);
     config.attrs = &attr;
-    config.numAttrs = down ? 1 : 0;
-    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, q, ring));
-  };
-  auto both = [&](auto tiles_tag) {
-    const int first = run(std::false_type{}, tiles_tag);
-    return first != 0 ? first : run(std::true_type{}, tiles_tag);
+    config.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, p, ring));
   };
   using std::integral_constant;
-  if (T <= 8) return both(integral_constant<int, 1>{});
-  if (T <= 16) return both(integral_constant<int, 2>{});
-  if (T <= 32) return both(integral_constant<int, 4>{});
-  return both(integral_constant<int, 8>{});
+  if (T <= 8) return run(integral_constant<int, 1>{});
+  if (T <= 16) return run(integral_constant<int, 2>{});
+  if (T <= 32) return run(integral_constant<int, 4>{});
+  return run(integral_constant<int, 8>{});
 }

@@ -715,7 +715,7 @@ int dm_select_experts_bwd(const void* logits, int logits_are_bf16, int64_t strid
                           int renormalize, float scale, const void* ids, int ids_are_int64, const void* grad_scores,
                           int scores_are_bf16, void* grad_logits, void* stream);
 
-/* dm_few_tokens: the whole layer for up to DM_FEW_TOKENS_MAX tokens with bf16 weights, all experts local, in two launches.
+/* dm_few_tokens: the whole layer for up to DM_FEW_TOKENS_MAX tokens with bf16 weights, all experts local, in one cooperative launch.
  * out[t] = sum_e c[t, e] W2[e] SwiGLU(W13[e] x[t]), c[t, e] = sum of the scores of token t's routes to expert e.  ids outside
  * [0, E) go nowhere, other than -1 they are reported in `status`.  D % 64 == 0, F % 8 == 0, E <= 1024, K <= 32.  The workspace
  * (dm_few_tokens_workspace_bytes, on the device of the launch; a negative DM_RC_* for an unsupported shape) is zeroed once before
