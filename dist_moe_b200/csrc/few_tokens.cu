@@ -43,6 +43,10 @@ constexpr int kFewMaxDepth = 12;
 constexpr int kFewRedFloats = kFewWarps * kFewRows * 8;
 constexpr int kFewQueue = 4;                   // tickets on their way from the weights' warp to the others
 constexpr int kFewTicketStrips = 3;            // strips for every block from which on blocks draw tickets
+__host__ __device__ constexpr int few_sum_bytes(int T) {
+  const int tile = 2 * kFewRedFloats * 4, by_token = kFewWarps * kFewRows * (T | 1) * 4;
+  return ((T > 8 && by_token > tile ? by_token : tile) + 15) / 16 * 16;
+}
 constexpr uint64_t kFewWaitNs = 2000000000ull;
 
 struct FewPhase {
@@ -383,6 +387,9 @@ __device__ __noinline__ void few_wait_on(uint64_t* bar, uint32_t parity, int* ab
 }
 
 // The warps that multiply.  kTiles: tiles of eight columns that the accumulators hold.  `turn`: which warps look after the next sums.
+// Columns are an expert's tokens, next to one another; W2, which sums over the experts, adds them to sums by token in shared memory at
+// the end of each expert's items.  Up to eight tokens are one tile anyhow: there W2's columns are the tokens themselves.  (With them as
+// columns at every size, 32 and 64 tokens of the layer below took 230 and 370 us.)
 template <bool kDown, int kTiles>
 __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, float* red,
                                              int* s_next, uint32_t zeros, int& turn) {
@@ -408,31 +415,28 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.f;
   };
-  // Columns.  W13: the expert's tokens; those beyond the last one repeat it and are not kept.  W2: all tokens, those that are not the
-  // expert's being zero.
+  constexpr bool kScatter = kDown && kTiles > 1, kByToken = kDown && kTiles == 1;
+  const int pitch = p.T | 1;  // of the sums by token
+  float* sums = red + warp * kFewRows * pitch;
+  auto clear_sums = [&] {
+    for (int i = lane; i < kFewRows * pitch; i += 32) sums[i] = 0.f;
+    __syncwarp();
+  };
   int tiles = 0;
-  int from[kTiles];  // offset of the column's row in a place, W2: -1 for none
-  uint32_t hit = 0;  // tiles that any token of the expert is in
+  int from[kTiles];  // offset of the column's row in a place, -1 for a token that is not the expert's
   auto columns = [&](int a) {
-    if (kDown) {
+    const int count = tab.base[a + 1] - tab.base[a];
+    if (kByToken) {
       const uint64_t tokens = tab.tokens[tab.expert[a]];
-      tiles = (p.T + 7) >> 3;
-      hit = 0;
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        const int t = 8 * n + g;
-        from[n] = (tokens >> t) & 1 ? __popcll(tokens & ((1ull << t) - 1)) * kFewRowPitch : -1;
-        hit |= ((tokens >> (8 * n)) & 0xff) != 0 ? 1u << n : 0u;
-      }
-    } else {
-      const int count = tab.base[a + 1] - tab.base[a];
+      tiles = 1;
+      from[0] = (tokens >> g) & 1 ? __popcll(tokens & ((1ull << g) - 1)) * kFewRowPitch : -1;
+    } else {  // columns beyond the last token repeat it, and are not kept
       tiles = (count + 7) >> 3;
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) from[n] = min(8 * n + g, count - 1) * kFewRowPitch;
-      hit = (1u << tiles) - 1;
     }
   };
-  // `n_items` items in a row; `first_alone`: no tile but the first is hit
+  // `n_items` items in a row; `first_alone`: one tile
   auto run = [&](int c, int n_items, auto first_alone) {
     int k = c * kFewStep + warp * 32;
 #pragma unroll 1
@@ -443,8 +447,8 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
         const uint4 lo0 = lds16(aw), hi0 = lds16(aw + up * 128), lo1 = lds16(aw + half * 128), hi1 = lds16(aw + (half + up) * 128);
 #pragma unroll
         for (int n = 0; n < (decltype(first_alone)::value ? 1 : kTiles); ++n) {
-          if (!decltype(first_alone)::value && ((hit >> n) & 1) == 0) continue;
-          const uint4 b = lds16(kDown && from[n] < 0 ? none : at_b + here + from[n]);
+          if (n >= tiles) break;
+          const uint4 b = lds16(kByToken && from[n] < 0 ? none : at_b + here + from[n]);
           mma_16x8x16(acc[0][n], lo0.x, hi0.x, lo0.y, hi0.y, b.x, b.y);
           mma_16x8x16(acc[1][n], lo1.x, hi1.x, lo1.y, hi1.y, b.x, b.y);
           mma_16x8x16(acc[0][n], lo0.z, hi0.z, lo0.w, hi0.w, b.z, b.w);
@@ -463,70 +467,60 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     }
   };
   clear();
+  if (kScatter) clear_sums();
   FewCursor<kDown> at = work.begin;
   int strip_no = 0;  // two places for the next ticket: a warp may still read one while the next strip's is written
   bool whole = at.c == 0 && (!kDown || at.a == 0);  // the strip from its first item on
   for (int left = work.items; left > 0;) {
     columns(at.a);
     const int n_items = min(left, work.steps - at.c);
-    if (kTiles == 1 || hit == 1)
+    if (kTiles == 1 || tiles == 1)
       run(at.c, n_items, std::true_type{});
     else
       run(at.c, n_items, std::false_type{});
     left -= n_items;
     const FewCursor<kDown> done = at;
+    const int base = tab.base[at.a], pairs = tab.base[at.a + 1] - base;
     at.c += n_items - 1;
     at.next(work.strips, active, work.steps);
+    if (kScatter) {
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        if (n >= tiles) break;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col = 8 * n + 2 * quad + j;
+          if (col < pairs) {
+            float* to = sums + tab.token[base + col] + rho * pitch;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              to[i * half * pitch] += acc[i][n][j];
+              to[(i * half + up) * pitch] += acc[i][n][2 + j];
+            }
+          }
+        }
+      }
+      clear();
+    }
     const bool strip_end = kDown ? at.strip != done.strip : at.c == 0;
     if (!strip_end && left > 0) continue;
-    // ---- sum over the warps, a tile at a time, in two buffers in turn: one barrier each.  The warps take turns at what follows it; the
-    // others go on with the next strip. ------------------------------------------------------------------------------
+    // ---- the strip's sums over the warps ---------------------------------------------------------------------------------
     whole = whole && strip_end;
-    const int base = tab.base[done.a], count = kDown ? p.T : tab.base[done.a + 1] - base;
-    constexpr int kOut = kDown ? kFewRows : 16;  // outputs of a column
-    int drawn = 0;
-#pragma unroll 1
-    for (int n = 0; n < tiles; ++n) {
-      float* buf = red + (turn & 1) * kFewRedFloats;
-      float* to = buf + (warp * kFewRows + rho) * 8 + 2 * quad;
-#pragma unroll
-      for (int m = 0; m < kTiles; ++m)
-        if (m == n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            *reinterpret_cast<float2*>(to + i * half * 8) = make_float2(acc[i][m][0], acc[i][m][1]);
-            *reinterpret_cast<float2*>(to + (i * half + up) * 8) = make_float2(acc[i][m][2], acc[i][m][3]);
-          }
-      if (work.tickets && n == 0 && warp == 0) {  // one warp decides for all: they stay together where the ticket does not come
-        const int next = queue.next(ring.abort_flag, lane);
-        if (lane == 0) s_next[strip_no & 1] = next < 0 ? 0x7fffffff : next;
-      }
-      multipliers_meet();
-      if (work.tickets && n == 0) drawn = s_next[strip_no & 1];
-      const int cols = min(count - 8 * n, 8);
-      const int slot = (warp + turn * (kOut * 8 / 32)) & (kFewWarps - 1);  // of 32 outputs
-      ++turn;
-      if (slot * 32 >= kOut * cols) continue;
-      const int o = slot * 32 + lane, r = o & (kOut - 1), col = 8 * n + o / kOut;
-      const bool in = o < kOut * cols;
-      float v = 0.f, u = 0.f;
-#pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) {
-        v += buf[(w * kFewRows + r) * 8 + (o / kOut)];
-        if (!kDown) u += buf[(w * kFewRows + 16 + r) * 8 + (o / kOut)];
-      }
+    // One warp, 32 outputs (place `slot` among the strip's), an output a lane: row r, column col, sums v, and u of up.
+    auto conclude = [&](int slot, int r, int col, bool in, float v, float u) {
       bool mine = true;  // to finish these outputs
       if (!whole) {
         const int64_t q = kDown ? done.strip : static_cast<int64_t>(done.a) * work.strips + done.strip;  // strip of the product
         const int first = work.split.first_block(q), last = work.split.last_block(q);
-        const int at_out = (8 * n * kOut + o) * (kDown ? 1 : 2);
-        auto part = [&](int block) { return phase.partial + work.split.place(block, q) * (kFewRows * 8 * kTiles) + at_out; };
+        auto part = [&](int block) {
+          return phase.partial + work.split.place(block, q) * (kFewRows * 8 * kTiles) + (slot * 32 + lane) * (kDown ? 1 : 2);
+        };
         if (kDown)
           __stcg(part(blockIdx.x), v);
         else
           __stcg(reinterpret_cast<float2*>(part(blockIdx.x)), make_float2(v, u));
         // every block's warp with these outputs arrives; the last one finds all parts there
-        int32_t* arrived = phase.arrived + (first * kTiles + n) * (kOut * 8 / 32) + slot;
+        int32_t* arrived = phase.arrived + first * 8 * kTiles + slot;
         __syncwarp();
         int before = 0;
         if (lane == 0) {
@@ -536,6 +530,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
         mine = __shfl_sync(0xffffffffu, before, 0) == last - first;
         if (mine) {
           v = u = 0.f;
+#pragma unroll 4
           for (int block = first; block <= last; ++block) {
             if (kDown) {
               v += __ldcg(part(block));
@@ -556,6 +551,52 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
           swiglu_f32(gate, up1, z, p.act);
           p.h[static_cast<int64_t>(base + col) * p.F + done.strip * 16 + r] = __float2bfloat16_rn(tab.share[base + col] * z[0]);
         }
+      }
+    };
+    int drawn = 0;
+    if (kScatter) {
+      multipliers_meet();
+      for (int col = warp; col < p.T; col += kFewWarps) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) v += red[(w * kFewRows + lane) * pitch + col];
+        conclude(col, lane, col, true, v, 0.f);
+      }
+      multipliers_meet();
+      clear_sums();
+    } else {
+      // A tile at a time, in two buffers in turn: one barrier each.  The warps take turns at what follows it; the others go on with the
+      // next strip.
+      constexpr int kOut = kDown ? kFewRows : 16;  // outputs of a column
+#pragma unroll 1
+      for (int n = 0; n < tiles; ++n) {
+        float* buf = red + (turn & 1) * kFewRedFloats;
+        float* to = buf + (warp * kFewRows + rho) * 8 + 2 * quad;
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m)
+          if (m == n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              *reinterpret_cast<float2*>(to + i * half * 8) = make_float2(acc[i][m][0], acc[i][m][1]);
+              *reinterpret_cast<float2*>(to + (i * half + up) * 8) = make_float2(acc[i][m][2], acc[i][m][3]);
+            }
+        if (work.tickets && n == 0 && warp == 0) {  // one warp decides for all: they stay together where the ticket does not come
+          const int next = queue.next(ring.abort_flag, lane);
+          if (lane == 0) s_next[strip_no & 1] = next < 0 ? 0x7fffffff : next;
+        }
+        multipliers_meet();
+        if (work.tickets && n == 0) drawn = s_next[strip_no & 1];
+        const int cols = min((kDown ? p.T : pairs) - 8 * n, 8);
+        const int o = ((warp + turn * (kOut * 8 / 32)) & (kFewWarps - 1)) * 32 + lane, r = o & (kOut - 1), col = o / kOut;
+        ++turn;
+        if (o - lane >= kOut * cols) continue;
+        float v = 0.f, u = 0.f;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) {
+          v += buf[(w * kFewRows + r) * 8 + col];
+          if (!kDown) u += buf[(w * kFewRows + 16 + r) * 8 + col];
+        }
+        conclude(n * (kOut * 8 / 32) + o / 32, r, 8 * n + col, o < kOut * cols, v, u);
       }
     }
     clear();
@@ -578,8 +619,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
   __shared__ uint64_t full[kFewMaxDepth], empty[kFewMaxDepth], queue_full[kFewQueue], queue_empty[kFewQueue];
   __shared__ int s_found[2], s_ticket[kFewQueue], s_next[2], abort_flag;
   __shared__ __align__(16) uint8_t zeros[kFewStep * 2];  // a row for the columns that an expert has none for
-  float* red = reinterpret_cast<float*>(smem + ring_bytes);  // [2][warps along the inner dimension][32 rows][8]
-  const FewTables tab(smem + ring_bytes + 2 * kFewRedFloats * 4, p.T, p.E, p.K);
+  float* red = reinterpret_cast<float*>(smem + ring_bytes);  // [2][warps][32 rows][8] of a tile; W2 [warps][32 rows][tokens]
+  const FewTables tab(smem + ring_bytes + few_sum_bytes(p.T), p.T, p.E, p.K);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == kFewWarps) {
     if (lane < kFewMaxDepth) {
@@ -739,8 +780,8 @@ extern "C" int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, 
   if (rc != kRcOk) return rc;
   auto run = [&](auto tiles_tag) {
     constexpr auto kernel = few_tokens_kernel<decltype(tiles_tag)::value>;
-    constexpr int most = 226 * 1024, red = 2 * kFewRedFloats * 4;
-    const int tables = FewTables::bytes(p.T, p.E, p.K);
+    constexpr int most = 226 * 1024;
+    const int red = few_sum_bytes(p.T), tables = FewTables::bytes(p.T, p.E, p.K);
     const int ring = (most - 1024 - red - tables) / 1024 * 1024;
     static PerDeviceOnce attr_set;
     const int arc = once_per_device(attr_set, [] {
