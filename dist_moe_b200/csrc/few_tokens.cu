@@ -13,8 +13,8 @@
 // A block works on strips of 32 weight rows (16 features of gate and up; 32 output columns); an item is 256 values of the inner
 // dimension of a strip, 16 KiB.  Where W13 has three strips or more for every block, blocks take them by tickets; else, and for W2, the
 // items of all strips are dealt out evenly over the blocks, whatever the number of experts hit.  A strip that is cut between blocks is
-// summed by the one of them that finishes last, in the order of the blocks.  The eight warps that multiply share an item's inner
-// dimension.
+// summed by the one of them that finishes last, in the order of the blocks.  Of the eight warps that multiply, four share an item's
+// inner dimension and two its rows.
 //
 // With so few columns the products are mma.sync m16n8k16, weights as the 16-row operand, tokens as the 8 columns: both operands are
 // then read 16 bytes a lane along the inner dimension as they lie in shared memory, its order inside 32 values being the same for both
@@ -31,21 +31,25 @@ namespace dm {
 constexpr int kFewTokens = DM_FEW_TOKENS_MAX;
 constexpr int kFewExperts = 1024;
 constexpr int kFewTopK = 32;
-constexpr int kFewWarps = 8;                               // that multiply, side by side along the inner dimension
+constexpr int kFewLineWarps = 4, kFewWarps = 2 * kFewLineWarps;  // that multiply: side by side along the inner dimension; all
 constexpr int kFewThreads = 32 * (kFewWarps + 2);          // and one that loads weights, one that loads rows of x or h
-constexpr int kFewStep = 32 * kFewWarps;                  // values of the inner dimension per item
-constexpr int kFewLines = kFewStep / 64;                   // 128-byte lines of an item's rows
+constexpr int kFewLines = kFewLineWarps;                   // 128-byte lines of an item's rows
+constexpr int kFewStep = 64 * kFewLines;                   // values of the inner dimension per item
 constexpr int kFewRows = 32;                               // weight rows per strip
 constexpr int kFewLineBytes = kFewRows * 128;
 constexpr int kFewWeightBytes = kFewLines * kFewLineBytes;  // weights of an item
 constexpr int kFewRowPitch = kFewStep * 2 + 64;  // rows of x or h: eight of them, 16 bytes a lane, hit every bank once
 constexpr int kFewMaxDepth = 12;
-constexpr int kFewRedFloats = kFewWarps * kFewRows * 8;
+constexpr int kFewColPitch = kFewRows + 4;                         // of a tile's sums: lanes of a store hit every bank once
+constexpr int kFewTileFloats = kFewLineWarps * 8 * kFewColPitch;    // of a tile, for every warp along the inner dimension
 constexpr int kFewQueue = 4;                   // tickets on their way from the weights' warp to the others
 constexpr int kFewTicketStrips = 3;            // strips for every block from which on blocks draw tickets
-__host__ __device__ constexpr int few_sum_bytes(int T) {
-  const int tile = 2 * kFewRedFloats * 4, by_token = kFewWarps * kFewRows * (T | 1) * 4;
-  return ((T > 8 && by_token > tile ? by_token : tile) + 15) / 16 * 16;
+__host__ __device__ constexpr int few_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8; }
+__host__ __device__ constexpr int few_chunk(int tiles) { return tiles < 4 ? tiles : 4; }  // tiles that meet at a time
+// Sums that meet in shared memory: two chunks of tiles in turn; W2 of more than one tile: all tokens.
+__host__ __device__ constexpr int few_sum_bytes(int T, int tiles) {
+  const int chunks = 2 * few_chunk(tiles) * kFewTileFloats * 4, by_token = kFewLineWarps * kFewRows * (T | 1) * 4;
+  return ((tiles > 1 && by_token > chunks ? by_token : chunks) + 15) / 16 * 16;
 }
 constexpr uint64_t kFewWaitNs = 2000000000ull;
 
@@ -389,37 +393,36 @@ __device__ __noinline__ void few_wait_on(uint64_t* bar, uint32_t parity, int* ab
 // The warps that multiply.  kTiles: tiles of eight columns that the accumulators hold.  `turn`: which warps look after the next sums.
 // Columns are an expert's tokens, next to one another; W2, which sums over the experts, adds them to sums by token in shared memory at
 // the end of each expert's items.  Up to eight tokens are one tile anyhow: there W2's columns are the tokens themselves.  (With them as
-// columns at every size, 32 and 64 tokens of the layer below took 230 and 370 us.)
+// columns at every size, 32 and 64 tokens of 64 experts x 2048 x 1408 took 230 and 370 us where 215 and 285 were reached.)
 template <bool kDown, int kTiles>
 __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, float* red,
                                              int* s_next, uint32_t zeros, int& turn) {
   FewWork<kDown> work(p, active);
   const FewPhase& phase = p.phase[kDown];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, quad = lane & 3;
+  const int g = lane >> 2, quad = lane & 3, line = warp & (kFewLineWarps - 1), half = warp / kFewLineWarps;
   const int rho = few_row(g);
-  // Rows of the lane: rho, rho + up and both with `half` more.  W13: rows 0 to 15 of an item are gate features, 16 to 31 those of up.
-  constexpr int half = kDown ? 16 : 8, up = kDown ? 8 : 16;
-  const uint32_t at_w = smem_u32(ring.base) + (warp >> 1) * kFewLineBytes + rho * 128 + ((((warp & 1) * 4 + quad) ^ rho) << 4);
-  const uint32_t at_b = smem_u32(ring.base) + kFewWeightBytes + warp * 64 + quad * 16;
-  const uint32_t none = zeros + warp * 64 + quad * 16;
+  // Rows of the lane: r0 and r0 + up.  W13: rows 0 to 15 of an item are gate features, 16 to 31 those of up.
+  constexpr int up = kDown ? 8 : 16;
+  const int r0 = half * (kDown ? 16 : 8) + rho;
+  const uint32_t at_w = smem_u32(ring.base) + line * kFewLineBytes + r0 * 128 + ((quad ^ rho) << 4);
+  const uint32_t at_b = smem_u32(ring.base) + kFewWeightBytes + line * 128 + quad * 16;
+  const uint32_t none = zeros + line * 128 + quad * 16;
   const uint32_t full0 = smem_u32(ring.full), empty0 = smem_u32(ring.empty);
   int place = ring.place;
   uint32_t round = ring.round, here = place * ring.place_bytes;
-  float acc[2][kTiles][4];
+  float acc[kTiles][4];
   auto clear = [&] {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.f;
+      for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
   };
   constexpr bool kScatter = kDown && kTiles > 1, kByToken = kDown && kTiles == 1;
   const int pitch = p.T | 1;  // of the sums by token
-  float* sums = red + warp * kFewRows * pitch;
+  float* sums = red + (line * kFewRows + 16 * half) * pitch;  // this warp's 16 rows
   auto clear_sums = [&] {
-    for (int i = lane; i < kFewRows * pitch; i += 32) sums[i] = 0.f;
+    for (int i = lane; i < 16 * pitch; i += 32) sums[i] = 0.f;
     __syncwarp();
   };
   int tiles = 0;
@@ -436,34 +439,80 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       for (int n = 0; n < kTiles; ++n) from[n] = min(8 * n + g, count - 1) * kFewRowPitch;
     }
   };
-  // `n_items` items in a row; `first_alone`: one tile
-  auto run = [&](int c, int n_items, auto first_alone) {
-    int k = c * kFewStep + warp * 32;
-#pragma unroll 1
-    for (int i = 0; i < n_items; ++i, k += kFewStep) {
-      if (!try_wait_addr(full0 + 8 * place, round)) few_wait_on(ring.full + place, round, ring.abort_flag, p.status);
-      if (k < work.inner) {  // beyond the last value weights and rows are zero
-        const uint32_t aw = at_w + here;
-        const uint4 lo0 = lds16(aw), hi0 = lds16(aw + up * 128), lo1 = lds16(aw + half * 128), hi1 = lds16(aw + (half + up) * 128);
+  // An item's operands; those of the next one are read while it is multiplied.
+  struct Operands {
+    uint4 lo[2], hi[2], b[2];
+  };
+  auto fetch = [&](Operands& x, bool in) {
+    if (!try_wait_addr(full0 + 8 * place, round)) few_wait_on(ring.full + place, round, ring.abort_flag, p.status);
+    if (in) {
 #pragma unroll
-        for (int n = 0; n < (decltype(first_alone)::value ? 1 : kTiles); ++n) {
-          if (n >= tiles) break;
-          const uint4 b = lds16(kByToken && from[n] < 0 ? none : at_b + here + from[n]);
-          mma_16x8x16(acc[0][n], lo0.x, hi0.x, lo0.y, hi0.y, b.x, b.y);
-          mma_16x8x16(acc[1][n], lo1.x, hi1.x, lo1.y, hi1.y, b.x, b.y);
-          mma_16x8x16(acc[0][n], lo0.z, hi0.z, lo0.w, hi0.w, b.z, b.w);
-          mma_16x8x16(acc[1][n], lo1.z, hi1.z, lo1.w, hi1.w, b.z, b.w);
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t aw = (at_w + here) ^ (h << 6);
+        x.lo[h] = lds16(aw);
+        x.hi[h] = lds16(aw + up * 128);
+        x.b[h] = lds16((kByToken && from[0] < 0 ? none : at_b + here + from[0]) + h * 64);
+      }
+    }
+  };
+  auto multiply = [&](const Operands& x, const uint4& b, int h, int n) {
+    mma_16x8x16(acc[n], x.lo[h].x, x.hi[h].x, x.lo[h].y, x.hi[h].y, b.x, b.y);
+    mma_16x8x16(acc[n], x.lo[h].z, x.hi[h].z, x.lo[h].w, x.hi[h].w, b.z, b.w);
+  };
+  auto leave = [&] {  // the item's place is read
+    __syncwarp();
+    if (lane == 0) arrive_addr(empty0 + 8 * place);
+    ++place;
+    here += ring.place_bytes;
+    if (place == ring.depth) {
+      place = 0;
+      here = 0;
+      round ^= 1u;
+    }
+  };
+  // `n_items` items in a row, `valid` of them with values for this warp: beyond the last line of weights a place holds anything.
+  auto run_one_tile = [&](int n_items, int valid) {
+    Operands x, y;
+    fetch(x, valid > 0);
+    leave();
+#pragma unroll 1
+    for (int i = 0; i < n_items; i += 2) {
+      if (i + 1 < n_items) {
+        fetch(y, i + 1 < valid);
+        leave();
+      }
+      if (i < valid) {
+        multiply(x, x.b[0], 0, 0);
+        multiply(x, x.b[1], 1, 0);
+      }
+      if (i + 1 >= n_items) break;
+      if (i + 2 < n_items) {
+        fetch(x, i + 2 < valid);
+        leave();
+      }
+      if (i + 1 < valid) {
+        multiply(y, y.b[0], 0, 0);
+        multiply(y, y.b[1], 1, 0);
+      }
+    }
+  };
+  auto run = [&](int n_items, int valid) {
+#pragma unroll 1
+    for (int i = 0; i < n_items; ++i) {
+      Operands x;
+      fetch(x, i < valid);
+      if (i < valid) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          multiply(x, x.b[h], h, 0);
+#pragma unroll
+          for (int n = 1; n < kTiles; ++n) {
+            if (n >= tiles) break;
+            multiply(x, lds16(at_b + here + from[n] + h * 64), h, n);
+          }
         }
       }
-      __syncwarp();
-      if (lane == 0) arrive_addr(empty0 + 8 * place);
-      ++place;
-      here += ring.place_bytes;
-      if (place == ring.depth) {
-        place = 0;
-        here = 0;
-        round ^= 1u;
-      }
+      leave();
     }
   };
   clear();
@@ -474,10 +523,11 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
   for (int left = work.items; left > 0;) {
     columns(at.a);
     const int n_items = min(left, work.steps - at.c);
+    const int valid = (work.inner - at.c * kFewStep - line * 64 + kFewStep - 1) / kFewStep;
     if (kTiles == 1 || tiles == 1)
-      run(at.c, n_items, std::true_type{});
+      run_one_tile(n_items, valid);
     else
-      run(at.c, n_items, std::false_type{});
+      run(n_items, valid);
     left -= n_items;
     const FewCursor<kDown> done = at;
     const int base = tab.base[at.a], pairs = tab.base[at.a + 1] - base;
@@ -492,66 +542,36 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
           const int col = 8 * n + 2 * quad + j;
           if (col < pairs) {
             float* to = sums + tab.token[base + col] + rho * pitch;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              to[i * half * pitch] += acc[i][n][j];
-              to[(i * half + up) * pitch] += acc[i][n][2 + j];
-            }
+            to[0] += acc[n][j];
+            to[up * pitch] += acc[n][2 + j];
           }
         }
       }
+      __syncwarp();
       clear();
     }
     const bool strip_end = kDown ? at.strip != done.strip : at.c == 0;
     if (!strip_end && left > 0) continue;
     // ---- the strip's sums over the warps ---------------------------------------------------------------------------------
     whole = whole && strip_end;
-    // One warp, 32 outputs (place `slot` among the strip's), an output a lane: row r, column col, sums v, and u of up.
-    auto conclude = [&](int slot, int r, int col, bool in, float v, float u) {
-      bool mine = true;  // to finish these outputs
-      if (!whole) {
-        const int64_t q = kDown ? done.strip : static_cast<int64_t>(done.a) * work.strips + done.strip;  // strip of the product
-        const int first = work.split.first_block(q), last = work.split.last_block(q);
-        auto part = [&](int block) {
-          return phase.partial + work.split.place(block, q) * (kFewRows * 8 * kTiles) + (slot * 32 + lane) * (kDown ? 1 : 2);
-        };
-        if (kDown)
-          __stcg(part(blockIdx.x), v);
-        else
-          __stcg(reinterpret_cast<float2*>(part(blockIdx.x)), make_float2(v, u));
-        // every block's warp with these outputs arrives; the last one finds all parts there
-        int32_t* arrived = phase.arrived + first * 8 * kTiles + slot;
-        __syncwarp();
-        int before = 0;
-        if (lane == 0) {
-          before = atom_add_acq_rel(arrived, 1);
-          if (before == last - first) *arrived = 0;  // clear for the next call
-        }
-        mine = __shfl_sync(0xffffffffu, before, 0) == last - first;
-        if (mine) {
-          v = u = 0.f;
-#pragma unroll 4
-          for (int block = first; block <= last; ++block) {
-            if (kDown) {
-              v += __ldcg(part(block));
-            } else {
-              const float2 vu = __ldcg(reinterpret_cast<const float2*>(part(block)));
-              v += vu.x;
-              u += vu.y;
-            }
-          }
-        }
+    // What the warps with the same outputs of a cut strip do in every block: store their parts, arrive, and the last one finds all parts.
+    const int64_t q = kDown ? done.strip : static_cast<int64_t>(done.a) * work.strips + done.strip;  // strip of the product
+    auto part = [&](int block, int o) {
+      return phase.partial + work.split.place(block, q) * (kFewRows * 8 * kTiles) + o * (kDown ? 1 : 2);
+    };
+    auto last_to_arrive = [&](int slot) {
+      const int first = work.split.first_block(q), others = work.split.last_block(q) - first;
+      int32_t* arrived = phase.arrived + first * 8 * kTiles + slot;
+      __syncwarp();
+      int before = 0;
+      if (lane == 0) {
+        before = atom_add_acq_rel(arrived, 1);
+        if (before == others) *arrived = 0;  // clear for the next call
       }
-      if (mine && in) {
-        if (kDown) {
-          p.out[static_cast<int64_t>(col) * p.D + done.strip * kFewRows + r] = __float2bfloat16_rn(v);
-        } else if (done.strip * 16 + r < p.F) {
-          const float gate[1] = {v}, up1[1] = {u};
-          float z[1];
-          swiglu_f32(gate, up1, z, p.act);
-          p.h[static_cast<int64_t>(base + col) * p.F + done.strip * 16 + r] = __float2bfloat16_rn(tab.share[base + col] * z[0]);
-        }
-      }
+      return __shfl_sync(0xffffffffu, before, 0) == others;
+    };
+    auto write_out = [&](int r, int col, float v) {
+      p.out[static_cast<int64_t>(col) * p.D + done.strip * kFewRows + r] = __float2bfloat16_rn(v);
     };
     int drawn = 0;
     if (kScatter) {
@@ -559,44 +579,95 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       for (int col = warp; col < p.T; col += kFewWarps) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) v += red[(w * kFewRows + lane) * pitch + col];
-        conclude(col, lane, col, true, v, 0.f);
+        for (int w = 0; w < kFewLineWarps; ++w) v += red[(w * kFewRows + lane) * pitch + col];
+        if (whole)
+          write_out(lane, col, v);
+        else
+          __stcg(part(blockIdx.x, col * kFewRows + lane), v);
+      }
+      if (!whole && last_to_arrive(warp)) {
+        const int first = work.split.first_block(q), last = work.split.last_block(q);
+        for (int col = warp; col < p.T; col += 4 * kFewWarps) {  // four columns of a block's part on their way at a time
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int block = first; block <= last; ++block) {
+            const float* from_block = part(block, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (col + i * kFewWarps < p.T) v[i] += __ldcg(from_block + (col + i * kFewWarps) * kFewRows);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (col + i * kFewWarps < p.T) write_out(lane, col + i * kFewWarps, v[i]);
+        }
       }
       multipliers_meet();
       clear_sums();
     } else {
-      // A tile at a time, in two buffers in turn: one barrier each.  The warps take turns at what follows it; the others go on with the
-      // next strip.
-      constexpr int kOut = kDown ? kFewRows : 16;  // outputs of a column
-#pragma unroll 1
-      for (int n = 0; n < tiles; ++n) {
-        float* buf = red + (turn & 1) * kFewRedFloats;
-        float* to = buf + (warp * kFewRows + rho) * 8 + 2 * quad;
+      // A chunk of tiles at a time, in two buffers in turn: one barrier each.  The warps take turns at what follows it; the others go on
+      // with the next strip.
+      constexpr int kChunk = few_chunk(kTiles), kOut = kDown ? kFewRows : 16;  // outputs of a column
 #pragma unroll
-        for (int m = 0; m < kTiles; ++m)
-          if (m == n)
+      for (int n0 = 0; n0 < kTiles; n0 += kChunk) {
+        if (n0 >= tiles) break;
+        float* buf = red + (turn & 1) * kChunk * kFewTileFloats;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              *reinterpret_cast<float2*>(to + i * half * 8) = make_float2(acc[i][m][0], acc[i][m][1]);
-              *reinterpret_cast<float2*>(to + (i * half + up) * 8) = make_float2(acc[i][m][2], acc[i][m][3]);
-            }
-        if (work.tickets && n == 0 && warp == 0) {  // one warp decides for all: they stay together where the ticket does not come
+        for (int n = 0; n < kChunk; ++n) {
+          if (n0 + n >= tiles) break;
+          float* to = buf + n * kFewTileFloats + (line * 8 + 2 * quad) * kFewColPitch + r0;
+          to[0] = acc[n0 + n][0];
+          to[kFewColPitch] = acc[n0 + n][1];
+          to[up] = acc[n0 + n][2];
+          to[kFewColPitch + up] = acc[n0 + n][3];
+        }
+        if (work.tickets && n0 == 0 && warp == 0) {  // one warp decides for all: they stay together where the ticket does not come
           const int next = queue.next(ring.abort_flag, lane);
           if (lane == 0) s_next[strip_no & 1] = next < 0 ? 0x7fffffff : next;
         }
         multipliers_meet();
-        if (work.tickets && n == 0) drawn = s_next[strip_no & 1];
-        const int cols = min((kDown ? p.T : pairs) - 8 * n, 8);
-        const int o = ((warp + turn * (kOut * 8 / 32)) & (kFewWarps - 1)) * 32 + lane, r = o & (kOut - 1), col = o / kOut;
-        ++turn;
-        if (o - lane >= kOut * cols) continue;
-        float v = 0.f, u = 0.f;
+        if (work.tickets && n0 == 0) drawn = s_next[strip_no & 1];
+        const int outs = kOut * min((kDown ? p.T : pairs) - 8 * n0, 8 * kChunk);
+        const int o0 = ((warp + (turn >> 1)) & (kFewWarps - 1)) * 32 + lane;
+        turn = (turn ^ 1) + 2 * ((outs + 31) / 32);  // the buffer in its last bit
+#pragma unroll 1
+        for (int o = o0; o - lane < outs; o += 32 * kFewWarps) {
+          const int r = o & (kOut - 1), col = o / kOut;
+          const float* of = buf + (col >> 3) * kFewTileFloats + (col & 7) * kFewColPitch + r;
+          float v = 0.f, u = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) {
-          v += buf[(w * kFewRows + r) * 8 + col];
-          if (!kDown) u += buf[(w * kFewRows + 16 + r) * 8 + col];
+          for (int w = 0; w < kFewLineWarps; ++w) {
+            v += of[w * 8 * kFewColPitch];
+            if (!kDown) u += of[w * 8 * kFewColPitch + 16];
+          }
+          if (!whole) {
+            const int at_out = n0 * kOut * 8 + o;
+            if (kDown)
+              __stcg(part(blockIdx.x, at_out), v);
+            else
+              __stcg(reinterpret_cast<float2*>(part(blockIdx.x, at_out)), make_float2(v, u));
+            if (!last_to_arrive(at_out / 32)) continue;
+            v = u = 0.f;
+            const int last = work.split.last_block(q);
+            for (int block = work.split.first_block(q); block <= last; ++block) {
+              if (kDown) {
+                v += __ldcg(part(block, at_out));
+              } else {
+                const float2 vu = __ldcg(reinterpret_cast<const float2*>(part(block, at_out)));
+                v += vu.x;
+                u += vu.y;
+              }
+            }
+          }
+          if (o >= outs) continue;
+          if (kDown) {
+            write_out(r, 8 * n0 + col, v);
+          } else if (done.strip * 16 + r < p.F) {
+            const float gate[1] = {v}, up1[1] = {u};
+            float z[1];
+            swiglu_f32(gate, up1, z, p.act);
+            const int pair = base + 8 * n0 + col;
+            p.h[static_cast<int64_t>(pair) * p.F + done.strip * 16 + r] = __float2bfloat16_rn(tab.share[pair] * z[0]);
+          }
         }
-        conclude(n * (kOut * 8 / 32) + o / 32, r, 8 * n + col, o < kOut * cols, v, u);
       }
     }
     clear();
@@ -618,9 +689,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
   uint8_t* smem = few_smem_raw + (-smem_u32(few_smem_raw) & 1023u);  // an offset: what lies there stays known as shared memory
   __shared__ uint64_t full[kFewMaxDepth], empty[kFewMaxDepth], queue_full[kFewQueue], queue_empty[kFewQueue];
   __shared__ int s_found[2], s_ticket[kFewQueue], s_next[2], abort_flag;
-  __shared__ __align__(16) uint8_t zeros[kFewStep * 2];  // a row for the columns that an expert has none for
-  float* red = reinterpret_cast<float*>(smem + ring_bytes);  // [2][warps][32 rows][8] of a tile; W2 [warps][32 rows][tokens]
-  const FewTables tab(smem + ring_bytes + few_sum_bytes(p.T), p.T, p.E, p.K);
+  __shared__ __align__(16) uint8_t zeros[kFewStep * 2 + 16];  // a row for the columns that an expert has none for
+  float* red = reinterpret_cast<float*>(smem + ring_bytes);
+  const FewTables tab(smem + ring_bytes + few_sum_bytes(p.T, kTiles), p.T, p.E, p.K);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == kFewWarps) {
     if (lane < kFewMaxDepth) {
@@ -718,7 +789,7 @@ struct FewLayout {
 };
 static FewLayout few_layout(int64_t T, int64_t F, int64_t K) {
   auto a128 = [](int64_t v) { return (v + 127) / 128 * 128; };
-  const int64_t blocks = sm_count(), tiles = T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8;
+  const int64_t blocks = sm_count(), tiles = few_tiles(static_cast<int>(T));
   const int64_t partial = a128(blocks * 2 * kFewRows * 8 * tiles * 4), arrived = a128(blocks * tiles * 8 * 4);
   FewLayout l;
   l.meeting = 0;
@@ -781,7 +852,7 @@ extern "C" int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, 
   auto run = [&](auto tiles_tag) {
     constexpr auto kernel = few_tokens_kernel<decltype(tiles_tag)::value>;
     constexpr int most = 226 * 1024;
-    const int red = few_sum_bytes(p.T), tables = FewTables::bytes(p.T, p.E, p.K);
+    const int red = few_sum_bytes(p.T, decltype(tiles_tag)::value), tables = FewTables::bytes(p.T, p.E, p.K);
     const int ring = (most - 1024 - red - tables) / 1024 * 1024;
     static PerDeviceOnce attr_set;
     const int arc = once_per_device(attr_set, [] {
