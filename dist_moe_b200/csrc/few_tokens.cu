@@ -10,16 +10,18 @@
 // another brings the rows of x or h that meet them (512 bytes by one cp.async of the warp) and alone waits for the other blocks where
 // h begins: by then 200 KB of W2 per SM are there.  All blocks are resident at once (cooperative launch), and that wait is bounded.
 //
-// A block works on strips of 32 weight rows (16 features of gate and up; 32 output columns); an item is 256 values of the inner
-// dimension of a strip, 16 KiB.  Where W13 has three strips or more for every block, blocks take them by tickets; else, and for W2, the
-// items of all strips are dealt out evenly over the blocks, whatever the number of experts hit.  A strip that is cut between blocks is
-// summed by the one of them that finishes last, in the order of the blocks.  Of the eight warps that multiply, four share an item's
-// inner dimension and two its rows.
+// A block works on strips of 64 weight rows (32 features of gate and up; 64 output columns), 16 for each of its four warps that multiply;
+// an item is 128 values of the inner dimension of a strip, 16 KiB.  A warp has its rows for itself, sums them in registers and ends a
+// strip without the others: nothing but the ring's places keeps the warps together.  (With the inner dimension of an item shared by
+// eight warps, the barrier and the sums in shared memory at the end of a strip stopped the stream: 32 tokens of 64 experts x 2048 x 1408
+// took 207 us, 176 without them.)  Where W13 has enough strips, blocks take them by tickets; else, and for W2, the items of all strips
+// are dealt out evenly over the blocks, whatever the number of experts hit.  Rows of a strip that is cut between blocks are summed by
+// the one of the blocks' warps that finishes last, in the order of the blocks.
 //
 // With so few columns the products are mma.sync m16n8k16, weights as the 16-row operand, tokens as the 8 columns: both operands are
 // then read 16 bytes a lane along the inner dimension as they lie in shared memory, its order inside 32 values being the same for both
 // (lane t of a row holds values 8 t .. 8 t + 7, in two instructions), and a gate value meets its up value in the same lane.  Row g of
-// the instruction is row few_row(g) of the tile, which keeps the reads of the 128-byte swizzle free of bank conflicts.
+// the instruction is row few_row(g) of the warp's rows, which keeps the reads of the 128-byte swizzle free of bank conflicts.
 #include <type_traits>
 
 #include "few_split.cuh"
@@ -31,33 +33,27 @@ namespace dm {
 constexpr int kFewTokens = DM_FEW_TOKENS_MAX;
 constexpr int kFewExperts = 1024;
 constexpr int kFewTopK = 32;
-constexpr int kFewLineWarps = 4, kFewWarps = 2 * kFewLineWarps;  // that multiply: side by side along the inner dimension; all
-constexpr int kFewThreads = 32 * (kFewWarps + 2);          // and one that loads weights, one that loads rows of x or h
-constexpr int kFewLines = kFewLineWarps;                   // 128-byte lines of an item's rows
-constexpr int kFewStep = 64 * kFewLines;                   // values of the inner dimension per item
-constexpr int kFewRows = 32;                               // weight rows per strip
+constexpr int kFewWarps = 4;                       // that multiply, 16 weight rows each
+constexpr int kFewThreads = 32 * (kFewWarps + 2);  // and one that loads weights, one that loads rows of x or h
+constexpr int kFewRows = 16 * kFewWarps;           // weight rows per strip
+constexpr int kFewFeatures = kFewRows / 2;         // of W13
+constexpr int kFewLines = 2;                       // 128-byte lines of an item's rows
+constexpr int kFewStep = 64 * kFewLines;           // values of the inner dimension per item
 constexpr int kFewLineBytes = kFewRows * 128;
 constexpr int kFewWeightBytes = kFewLines * kFewLineBytes;  // weights of an item
-constexpr int kFewRowPitch = kFewStep * 2 + 64;  // rows of x or h: eight of them, 16 bytes a lane, hit every bank once
-constexpr int kFewMaxDepth = 12;
-constexpr int kFewColPitch = kFewRows + 4;                         // of a tile's sums: lanes of a store hit every bank once
-constexpr int kFewTileFloats = kFewLineWarps * 8 * kFewColPitch;    // of a tile, for every warp along the inner dimension
-constexpr int kFewQueue = 4;                   // tickets on their way from the weights' warp to the others
-constexpr int kFewTicketStrips = 3;            // strips for every block from which on blocks draw tickets
+constexpr int kFewRowPitch = kFewStep * 2 + 64;    // rows of x or h: eight of them, 16 bytes a lane, hit every bank once
+constexpr int kFewMaxDepth = 13;
+constexpr int kFewQueue = 4;                       // tickets on their way from the weights' warp to the others
 __host__ __device__ constexpr int few_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8; }
-__host__ __device__ constexpr int few_chunk(int tiles) { return tiles < 4 ? tiles : 4; }  // tiles that meet at a time
-// Sums that meet in shared memory: two chunks of tiles in turn; W2 of more than one tile: all tokens.
-__host__ __device__ constexpr int few_sum_bytes(int T, int tiles) {
-  const int chunks = 2 * few_chunk(tiles) * kFewTileFloats * 4, by_token = kFewLineWarps * kFewRows * (T | 1) * 4;
-  return ((tiles > 1 && by_token > chunks ? by_token : chunks) + 15) / 16 * 16;
-}
+// W2 of more than one tile: a sum for every row and token.
+__host__ __device__ constexpr int few_sum_bytes(int T, int tiles) { return tiles > 1 ? (kFewRows * (T | 1) * 4 + 15) / 16 * 16 : 0; }
 constexpr uint64_t kFewWaitNs = 2000000000ull;
 
 struct FewPhase {
   CUtensorMap items;  // W13 (64 values, features, gate | up, lines, experts) or W2 (64 values, columns, lines, experts)
   CUtensorMap tail;   // W2 with a last line of fewer than 64 values: (values, columns, experts)
-  float* partial;     // [blocks][2][kFewRows * 8 * tiles]
-  int32_t* arrived;   // [blocks][tiles][8 or 4 warps' outputs], clear between calls
+  float* partial;     // [blocks][2][warps][tiles][32 lanes][4]
+  int32_t* arrived;   // [blocks][warps], clear between calls
 };
 struct FewParams {
   FewPhase phase[2];  // W13, W2
@@ -67,7 +63,7 @@ struct FewParams {
   int ids_are_int64, scores_are_bf16;
   __nv_bfloat16* h;  // [pairs of expert and token][F]
   __nv_bfloat16* out;
-  int32_t* meeting;  // blocks that have written their share of h; blocks that have seen it; tickets drawn.  Clear between calls
+  int32_t* meeting;  // warps that have written their share of h; blocks that have seen it; tickets drawn.  Clear between calls
   int T, D, F, E, K;
   ActParams act;
   int* status;
@@ -234,6 +230,9 @@ struct FewCursor {
   }
 };
 
+// Whole strips by tickets, where the last round of them is full enough.
+__device__ __forceinline__ bool few_by_tickets(int strips, int blocks) { return 5 * strips >= 4 * blocks * ((strips + blocks - 1) / blocks); }
+
 // What the warps of a block know of one of the two products.
 template <bool kDown>
 struct FewWork {
@@ -244,13 +243,13 @@ struct FewWork {
   __device__ __forceinline__ FewWork(const FewParams& p, int active)
       : inner(kDown ? p.F : p.D),
         steps((inner + kFewStep - 1) / kFewStep),
-        strips(kDown ? p.D / kFewRows : (p.F + 15) / 16),  // W13: of one expert
+        strips(kDown ? p.D / kFewRows : (p.F + kFewFeatures - 1) / kFewFeatures),  // W13: of one expert
         length(kDown ? active * steps : steps),            // items of a strip
         split(kDown ? strips : static_cast<int64_t>(active) * strips, length, gridDim.x) {
     const int64_t first = split.begin(blockIdx.x);
     items = static_cast<int>(split.end(blockIdx.x) - first);
     begin.set(0, 1, 1, 1);
-    tickets = !kDown && active * strips >= kFewTicketStrips * static_cast<int>(gridDim.x);
+    tickets = !kDown && few_by_tickets(active * strips, gridDim.x);
     if (tickets)
       draw(blockIdx.x, active);
     else if (items > 0)
@@ -323,7 +322,7 @@ __device__ __forceinline__ bool few_load_weights(const FewParams& p, const FewTa
           if (kDown)
             tma_load_4d(to, &phase.items, 0, strip * kFewRows, c * kFewLines, e, full);
           else
-            tma_load_5d(to, &phase.items, 0, strip * 16, 0, c * kFewLines, e, full);
+            tma_load_5d(to, &phase.items, 0, strip * kFewFeatures, 0, c * kFewLines, e, full);
         }
       }
       __syncwarp();
@@ -347,18 +346,19 @@ __device__ __forceinline__ bool few_load_weights(const FewParams& p, const FewTa
 template <bool kDown>
 __device__ __forceinline__ bool few_load_rows(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, int lane) {
   FewWork<kDown> work(p, active);
-  const uint32_t own = smem_u32(ring.base) + kFewWeightBytes + lane * 16;
+  const int piece = lane & 15, first = lane >> 4;  // 16 lanes a row
+  const uint32_t own = smem_u32(ring.base) + kFewWeightBytes + piece * 16;
   while (true) {
     FewCursor<kDown> at = work.begin;
     for (int i = 0; i < work.items; ++i) {
       if (!warp_mbar_wait(&ring.empty[ring.place], ring.round ^ 1u, ring.abort_flag)) return false;
-      const int k = at.c * kFewStep + lane * 8;
+      const int k = at.c * kFewStep + piece * 8;
       const bool in = k < work.inner;
       const int base = tab.base[at.a], count = tab.base[at.a + 1] - base;
       const __nv_bfloat16* source = (kDown ? p.h + static_cast<int64_t>(base) * work.inner : p.x) + (in ? k : 0);
       const uint32_t to = own + ring.place * ring.place_bytes;
 #pragma unroll 4
-      for (int j = 0; j < count; ++j)
+      for (int j = first; j < count; j += 2)
         cp_async16(to + j * kFewRowPitch, source + static_cast<int64_t>(kDown ? j : tab.token[base + j]) * work.inner, in);
       cp_async_arrive(&ring.full[ring.place]);
       at.next(work.strips, active, work.steps);
@@ -390,24 +390,24 @@ __device__ __noinline__ void few_wait_on(uint64_t* bar, uint32_t parity, int* ab
   if (!mbar_wait(bar, parity, abort_flag)) set_status(status, kPipelineTimeout, 7, blockIdx.x);
 }
 
-// The warps that multiply.  kTiles: tiles of eight columns that the accumulators hold.  `turn`: which warps look after the next sums.
-// Columns are an expert's tokens, next to one another; W2, which sums over the experts, adds them to sums by token in shared memory at
-// the end of each expert's items.  Up to eight tokens are one tile anyhow: there W2's columns are the tokens themselves.  (With them as
-// columns at every size, 32 and 64 tokens of 64 experts x 2048 x 1408 took 230 and 370 us where 215 and 285 were reached.)
+// The warps that multiply.  kTiles: tiles of eight columns that the accumulators hold.  Columns are an expert's tokens, next to one
+// another; W2, which sums over the experts, adds them to sums by token in shared memory at the end of each expert's items.  Up to eight
+// tokens are one tile anyhow: there W2's columns are the tokens themselves.  (With them as columns at every size, 32 and 64 tokens of the
+// layer above took 230 and 370 us where 215 and 285 were reached.)
 template <bool kDown, int kTiles>
-__device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, float* red,
-                                             int* s_next, uint32_t zeros, int& turn) {
+__device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, float* all_sums,
+                                             uint32_t zeros) {
   FewWork<kDown> work(p, active);
   const FewPhase& phase = p.phase[kDown];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, quad = lane & 3, line = warp & (kFewLineWarps - 1), half = warp / kFewLineWarps;
+  const int g = lane >> 2, quad = lane & 3;
   const int rho = few_row(g);
-  // Rows of the lane: r0 and r0 + up.  W13: rows 0 to 15 of an item are gate features, 16 to 31 those of up.
-  constexpr int up = kDown ? 8 : 16;
-  const int r0 = half * (kDown ? 16 : 8) + rho;
-  const uint32_t at_w = smem_u32(ring.base) + line * kFewLineBytes + r0 * 128 + ((quad ^ rho) << 4);
-  const uint32_t at_b = smem_u32(ring.base) + kFewWeightBytes + line * 128 + quad * 16;
-  const uint32_t none = zeros + line * 128 + quad * 16;
+  // Rows of the lane: r0 and r0 + up.  W13: the first half of a strip's rows are gate features, the second the same features of up.
+  constexpr int up = kDown ? 8 : kFewFeatures;
+  const int r0 = warp * (kDown ? 16 : 8) + rho;
+  const uint32_t at_w = smem_u32(ring.base) + r0 * 128 + ((quad ^ rho) << 4);
+  const uint32_t at_b = smem_u32(ring.base) + kFewWeightBytes + quad * 16;
+  const uint32_t none = zeros + quad * 16;
   const uint32_t full0 = smem_u32(ring.full), empty0 = smem_u32(ring.empty);
   int place = ring.place;
   uint32_t round = ring.round, here = place * ring.place_bytes;
@@ -419,8 +419,8 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
   };
   constexpr bool kScatter = kDown && kTiles > 1, kByToken = kDown && kTiles == 1;
-  const int pitch = p.T | 1;  // of the sums by token
-  float* sums = red + (line * kFewRows + 16 * half) * pitch;  // this warp's 16 rows
+  const int pitch = p.T | 1;
+  float* sums = all_sums + warp * 16 * pitch;  // of this warp's rows, by token
   auto clear_sums = [&] {
     for (int i = lane; i < 16 * pitch; i += 32) sums[i] = 0.f;
     __syncwarp();
@@ -439,25 +439,25 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       for (int n = 0; n < kTiles; ++n) from[n] = min(8 * n + g, count - 1) * kFewRowPitch;
     }
   };
-  // An item's operands; those of the next one are read while it is multiplied.
+  // A line's operands.
   struct Operands {
     uint4 lo[2], hi[2], b[2];
   };
-  auto fetch = [&](Operands& x, bool in) {
+  auto wait = [&] {
     if (!try_wait_addr(full0 + 8 * place, round)) few_wait_on(ring.full + place, round, ring.abort_flag, p.status);
-    if (in) {
+  };
+  auto fetch = [&](Operands& x, int line) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t aw = (at_w + here) ^ (h << 6);
-        x.lo[h] = lds16(aw);
-        x.hi[h] = lds16(aw + up * 128);
-        x.b[h] = lds16((kByToken && from[0] < 0 ? none : at_b + here + from[0]) + h * 64);
-      }
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t aw = (at_w + here + line * kFewLineBytes) ^ (h << 6);
+      x.lo[h] = lds16(aw);
+      x.hi[h] = lds16(aw + up * 128);
+      x.b[h] = lds16((kByToken && from[0] < 0 ? none : at_b + here + from[0]) + line * 128 + h * 64);
     }
   };
-  auto multiply = [&](const Operands& x, const uint4& b, int h, int n) {
-    mma_16x8x16(acc[n], x.lo[h].x, x.hi[h].x, x.lo[h].y, x.hi[h].y, b.x, b.y);
-    mma_16x8x16(acc[n], x.lo[h].z, x.hi[h].z, x.lo[h].w, x.hi[h].w, b.z, b.w);
+  auto multiply = [&](float (&to)[4], const Operands& x, const uint4& b, int h) {
+    mma_16x8x16(to, x.lo[h].x, x.hi[h].x, x.lo[h].y, x.hi[h].y, b.x, b.y);
+    mma_16x8x16(to, x.lo[h].z, x.hi[h].z, x.lo[h].w, x.hi[h].w, b.z, b.w);
   };
   auto leave = [&] {  // the item's place is read
     __syncwarp();
@@ -470,45 +470,41 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       round ^= 1u;
     }
   };
-  // `n_items` items in a row, `valid` of them with values for this warp: beyond the last line of weights a place holds anything.
-  auto run_one_tile = [&](int n_items, int valid) {
+  // `n_items` items in a row with `lines` lines of values.  Beyond them a place holds anything; in the last one zeros follow the values.
+  auto run_one_tile = [&](int n_items, int lines) {
+    float odd[4] = {0.f, 0.f, 0.f, 0.f};  // a chain of its own for every second line
     Operands x, y;
-    fetch(x, valid > 0);
-    leave();
 #pragma unroll 1
-    for (int i = 0; i < n_items; i += 2) {
-      if (i + 1 < n_items) {
-        fetch(y, i + 1 < valid);
-        leave();
-      }
-      if (i < valid) {
-        multiply(x, x.b[0], 0, 0);
-        multiply(x, x.b[1], 1, 0);
-      }
-      if (i + 1 >= n_items) break;
-      if (i + 2 < n_items) {
-        fetch(x, i + 2 < valid);
-        leave();
-      }
-      if (i + 1 < valid) {
-        multiply(y, y.b[0], 0, 0);
-        multiply(y, y.b[1], 1, 0);
+    for (int i = 0; i < n_items; ++i, lines -= kFewLines) {
+      wait();
+      fetch(x, 0);
+      if (lines > 1) fetch(y, 1);
+      leave();
+      multiply(acc[0], x, x.b[0], 0);
+      multiply(acc[0], x, x.b[1], 1);
+      if (lines > 1) {
+        multiply(odd, y, y.b[0], 0);
+        multiply(odd, y, y.b[1], 1);
       }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[0][j] += odd[j];
   };
-  auto run = [&](int n_items, int valid) {
+  auto run = [&](int n_items, int lines) {
 #pragma unroll 1
-    for (int i = 0; i < n_items; ++i) {
-      Operands x;
-      fetch(x, i < valid);
-      if (i < valid) {
+    for (int i = 0; i < n_items; ++i, lines -= kFewLines) {
+      wait();
+#pragma unroll 1
+      for (int line = 0; line < min(lines, kFewLines); ++line) {
+        Operands x;
+        fetch(x, line);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          multiply(x, x.b[h], h, 0);
+          multiply(acc[0], x, x.b[h], h);
 #pragma unroll
           for (int n = 1; n < kTiles; ++n) {
             if (n >= tiles) break;
-            multiply(x, lds16(at_b + here + from[n] + h * 64), h, n);
+            multiply(acc[n], x, lds16(at_b + here + from[n] + line * 128 + h * 64), h);
           }
         }
       }
@@ -518,16 +514,15 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
   clear();
   if (kScatter) clear_sums();
   FewCursor<kDown> at = work.begin;
-  int strip_no = 0;  // two places for the next ticket: a warp may still read one while the next strip's is written
   bool whole = at.c == 0 && (!kDown || at.a == 0);  // the strip from its first item on
   for (int left = work.items; left > 0;) {
     columns(at.a);
     const int n_items = min(left, work.steps - at.c);
-    const int valid = (work.inner - at.c * kFewStep - line * 64 + kFewStep - 1) / kFewStep;
+    const int lines = (work.inner - at.c * kFewStep + 63) / 64;
     if (kTiles == 1 || tiles == 1)
-      run_one_tile(n_items, valid);
+      run_one_tile(n_items, lines);
     else
-      run(n_items, valid);
+      run(n_items, lines);
     left -= n_items;
     const FewCursor<kDown> done = at;
     const int base = tab.base[at.a], pairs = tab.base[at.a + 1] - base;
@@ -552,129 +547,99 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     }
     const bool strip_end = kDown ? at.strip != done.strip : at.c == 0;
     if (!strip_end && left > 0) continue;
-    // ---- the strip's sums over the warps ---------------------------------------------------------------------------------
-    whole = whole && strip_end;
-    // What the warps with the same outputs of a cut strip do in every block: store their parts, arrive, and the last one finds all parts.
-    const int64_t q = kDown ? done.strip : static_cast<int64_t>(done.a) * work.strips + done.strip;  // strip of the product
-    auto part = [&](int block, int o) {
-      return phase.partial + work.split.place(block, q) * (kFewRows * 8 * kTiles) + o * (kDown ? 1 : 2);
-    };
-    auto last_to_arrive = [&](int slot) {
-      const int first = work.split.first_block(q), others = work.split.last_block(q) - first;
-      int32_t* arrived = phase.arrived + first * 8 * kTiles + slot;
+    // ---- the end of the strip, or of the block's part of it ------------------------------------------------------------------
+    bool mine = true;  // to finish these rows
+    if (!(whole && strip_end)) {
+      // What the warps with the same rows do in every block: store their parts, arrive, and the last one finds all parts.
+      const int64_t q = kDown ? done.strip : static_cast<int64_t>(done.a) * work.strips + done.strip;  // strip of the product
+      const int first = work.split.first_block(q), last = work.split.last_block(q);
+      auto part = [&](int block) {
+        return reinterpret_cast<float4*>(phase.partial) + ((work.split.place(block, q) * kFewWarps + warp) * kTiles) * 32 + lane;
+      };
+      auto value = [&](int n) {  // sums: lane's row and four tokens after another
+        if (!kScatter) return make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+        const float* of = sums + (lane & 15) * pitch;
+        const int t = 8 * n + 4 * (lane >> 4);
+        return make_float4(t < p.T ? of[t] : 0.f, t + 1 < p.T ? of[t + 1] : 0.f, t + 2 < p.T ? of[t + 2] : 0.f, t + 3 < p.T ? of[t + 3] : 0.f);
+      };
+      const int used = kScatter ? (p.T + 7) >> 3 : tiles;
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+        if (n < used) __stcg(part(blockIdx.x) + n * 32, value(n));
       __syncwarp();
       int before = 0;
       if (lane == 0) {
+        int32_t* arrived = phase.arrived + first * kFewWarps + warp;
         before = atom_add_acq_rel(arrived, 1);
-        if (before == others) *arrived = 0;  // clear for the next call
+        if (before == last - first) *arrived = 0;  // clear for the next call
       }
-      return __shfl_sync(0xffffffffu, before, 0) == others;
-    };
-    auto write_out = [&](int r, int col, float v) {
-      p.out[static_cast<int64_t>(col) * p.D + done.strip * kFewRows + r] = __float2bfloat16_rn(v);
-    };
-    int drawn = 0;
-    if (kScatter) {
-      multipliers_meet();
-      for (int col = warp; col < p.T; col += kFewWarps) {
-        float v = 0.f;
+      mine = __shfl_sync(0xffffffffu, before, 0) == last - first;
+      if (mine) {
+        float4 v[kTiles];
 #pragma unroll
-        for (int w = 0; w < kFewLineWarps; ++w) v += red[(w * kFewRows + lane) * pitch + col];
-        if (whole)
-          write_out(lane, col, v);
-        else
-          __stcg(part(blockIdx.x, col * kFewRows + lane), v);
-      }
-      if (!whole && last_to_arrive(warp)) {
-        const int first = work.split.first_block(q), last = work.split.last_block(q);
-        for (int col = warp; col < p.T; col += 4 * kFewWarps) {  // four columns of a block's part on their way at a time
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int block = first; block <= last; ++block) {
-            const float* from_block = part(block, lane);
+        for (int n = 0; n < kTiles; ++n) v[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int block = first; block <= last; ++block) {
+          const float4* theirs = part(block);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (col + i * kFewWarps < p.T) v[i] += __ldcg(from_block + (col + i * kFewWarps) * kFewRows);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (col + i * kFewWarps < p.T) write_out(lane, col + i * kFewWarps, v[i]);
-        }
-      }
-      multipliers_meet();
-      clear_sums();
-    } else {
-      // A chunk of tiles at a time, in two buffers in turn: one barrier each.  The warps take turns at what follows it; the others go on
-      // with the next strip.
-      constexpr int kChunk = few_chunk(kTiles), kOut = kDown ? kFewRows : 16;  // outputs of a column
-#pragma unroll
-      for (int n0 = 0; n0 < kTiles; n0 += kChunk) {
-        if (n0 >= tiles) break;
-        float* buf = red + (turn & 1) * kChunk * kFewTileFloats;
-#pragma unroll
-        for (int n = 0; n < kChunk; ++n) {
-          if (n0 + n >= tiles) break;
-          float* to = buf + n * kFewTileFloats + (line * 8 + 2 * quad) * kFewColPitch + r0;
-          to[0] = acc[n0 + n][0];
-          to[kFewColPitch] = acc[n0 + n][1];
-          to[up] = acc[n0 + n][2];
-          to[kFewColPitch + up] = acc[n0 + n][3];
-        }
-        if (work.tickets && n0 == 0 && warp == 0) {  // one warp decides for all: they stay together where the ticket does not come
-          const int next = queue.next(ring.abort_flag, lane);
-          if (lane == 0) s_next[strip_no & 1] = next < 0 ? 0x7fffffff : next;
-        }
-        multipliers_meet();
-        if (work.tickets && n0 == 0) drawn = s_next[strip_no & 1];
-        const int outs = kOut * min((kDown ? p.T : pairs) - 8 * n0, 8 * kChunk);
-        const int o0 = ((warp + (turn >> 1)) & (kFewWarps - 1)) * 32 + lane;
-        turn = (turn ^ 1) + 2 * ((outs + 31) / 32);  // the buffer in its last bit
-#pragma unroll 1
-        for (int o = o0; o - lane < outs; o += 32 * kFewWarps) {
-          const int r = o & (kOut - 1), col = o / kOut;
-          const float* of = buf + (col >> 3) * kFewTileFloats + (col & 7) * kFewColPitch + r;
-          float v = 0.f, u = 0.f;
-#pragma unroll
-          for (int w = 0; w < kFewLineWarps; ++w) {
-            v += of[w * 8 * kFewColPitch];
-            if (!kDown) u += of[w * 8 * kFewColPitch + 16];
-          }
-          if (!whole) {
-            const int at_out = n0 * kOut * 8 + o;
-            if (kDown)
-              __stcg(part(blockIdx.x, at_out), v);
-            else
-              __stcg(reinterpret_cast<float2*>(part(blockIdx.x, at_out)), make_float2(v, u));
-            if (!last_to_arrive(at_out / 32)) continue;
-            v = u = 0.f;
-            const int last = work.split.last_block(q);
-            for (int block = work.split.first_block(q); block <= last; ++block) {
-              if (kDown) {
-                v += __ldcg(part(block, at_out));
-              } else {
-                const float2 vu = __ldcg(reinterpret_cast<const float2*>(part(block, at_out)));
-                v += vu.x;
-                u += vu.y;
-              }
+          for (int n = 0; n < kTiles; ++n)
+            if (n < used) {
+              const float4 add = __ldcg(theirs + n * 32);
+              v[n].x += add.x, v[n].y += add.y, v[n].z += add.z, v[n].w += add.w;
             }
+        }
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          if (!kScatter) {
+            acc[n][0] = v[n].x, acc[n][1] = v[n].y, acc[n][2] = v[n].z, acc[n][3] = v[n].w;
+          } else if (n < used) {
+            float* of = sums + (lane & 15) * pitch;
+            const int t = 8 * n + 4 * (lane >> 4);
+            if (t < p.T) of[t] = v[n].x;
+            if (t + 1 < p.T) of[t + 1] = v[n].y;
+            if (t + 2 < p.T) of[t + 2] = v[n].z;
+            if (t + 3 < p.T) of[t + 3] = v[n].w;
           }
-          if (o >= outs) continue;
-          if (kDown) {
-            write_out(r, 8 * n0 + col, v);
-          } else if (done.strip * 16 + r < p.F) {
-            const float gate[1] = {v}, up1[1] = {u};
-            float z[1];
-            swiglu_f32(gate, up1, z, p.act);
-            const int pair = base + 8 * n0 + col;
-            p.h[static_cast<int64_t>(pair) * p.F + done.strip * 16 + r] = __float2bfloat16_rn(tab.share[pair] * z[0]);
+        }
+        __syncwarp();
+      }
+    }
+    if (mine) {
+      if (kScatter) {
+        __nv_bfloat16* to = p.out + done.strip * kFewRows + warp * 16 + (lane & 15);
+        for (int t = lane >> 4; t < p.T; t += 2) to[static_cast<int64_t>(t) * p.D] = __float2bfloat16_rn(sums[(lane & 15) * pitch + t]);
+      } else if (kByToken) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (2 * quad + j < p.T) {
+            __nv_bfloat16* to = p.out + static_cast<int64_t>(2 * quad + j) * p.D + done.strip * kFewRows + r0;
+            to[0] = __float2bfloat16_rn(acc[0][j]);
+            to[up] = __float2bfloat16_rn(acc[0][2 + j]);
+          }
+      } else if (done.strip * kFewFeatures + r0 < p.F) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          if (n >= tiles) break;
+          const float gate[2] = {acc[n][0], acc[n][1]}, up1[2] = {acc[n][2], acc[n][3]};
+          float z[2];
+          swiglu_f32(gate, up1, z, p.act);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = 8 * n + 2 * quad + j;
+            if (col < pairs)
+              p.h[static_cast<int64_t>(base + col) * p.F + done.strip * kFewFeatures + r0] = __float2bfloat16_rn(tab.share[base + col] * z[j]);
           }
         }
       }
     }
+    if (kScatter) {
+      __syncwarp();
+      clear_sums();
+    }
     clear();
     whole = true;
     if (work.tickets) {
-      ++strip_no;
-      work.draw(drawn, active);
+      const int next = queue.next(ring.abort_flag, lane);
+      work.draw(next < 0 ? 0x7fffffff : next, active);
       at = work.begin;
       left = work.items;
     }
@@ -688,9 +653,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
   extern __shared__ __align__(1024) uint8_t few_smem_raw[];
   uint8_t* smem = few_smem_raw + (-smem_u32(few_smem_raw) & 1023u);  // an offset: what lies there stays known as shared memory
   __shared__ uint64_t full[kFewMaxDepth], empty[kFewMaxDepth], queue_full[kFewQueue], queue_empty[kFewQueue];
-  __shared__ int s_found[2], s_ticket[kFewQueue], s_next[2], abort_flag;
+  __shared__ int s_found[2], s_ticket[kFewQueue], abort_flag;
   __shared__ __align__(16) uint8_t zeros[kFewStep * 2 + 16];  // a row for the columns that an expert has none for
-  float* red = reinterpret_cast<float*>(smem + ring_bytes);
+  float* sums = reinterpret_cast<float*>(smem + ring_bytes);
   const FewTables tab(smem + ring_bytes + few_sum_bytes(p.T, kTiles), p.T, p.E, p.K);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == kFewWarps) {
@@ -700,7 +665,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
     }
     if (lane < kFewQueue) {
       mbar_init(&queue_full[lane], 1);
-      mbar_init(&queue_empty[lane], 2);  // the rows' warp and one for those that multiply
+      mbar_init(&queue_empty[lane], 1 + kFewWarps);  // the rows' warp and those that multiply
     }
     if (lane == 0) {
       abort_flag = 0;
@@ -737,7 +702,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
     if (ok) {  // until h is there
       const uint64_t t0 = globaltimer_ns();
       uint32_t spins = 0;
-      while (ok && ld_acquire_gpu(p.meeting) < static_cast<int>(gridDim.x))
+      while (ok && ld_acquire_gpu(p.meeting) < static_cast<int>(gridDim.x) * kFewWarps)
         if ((++spins & 0xff) == 0 && (*const_cast<volatile int*>(&abort_flag) != 0 || globaltimer_ns() - t0 > kFewWaitNs)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       // the last one to leave clears them for the next call: every block has drawn its last ticket
@@ -751,22 +716,22 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
-    for (int i = threadIdx.x; i < tab.base[active]; i += 32 * kFewWarps) {  // read behind the first strip's barrier
+    for (int i = threadIdx.x; i < tab.base[active]; i += 32 * kFewWarps) {
       const int t = tab.token[i], e = tab.expert[tab.owner[i]];
       float share = 0.f;
       for (int k = 0; k < p.K; ++k)
         if (tab.id[t * p.K + k] == e) share += tab.score[t * p.K + k];
       tab.share[i] = share;
     }
-    int turn = 0;
-    few_multiply<false, kTiles>(p, tab, ring, queue, active, red, s_next, smem_u32(zeros), turn);
-    multipliers_meet();  // the block's share of h is written
-    if (threadIdx.x == 0) red_release_gpu_add(p.meeting, 1);
-    few_multiply<true, kTiles>(p, tab, ring, queue, active, red, s_next, smem_u32(zeros), turn);
+    multipliers_meet();  // shares are there
+    few_multiply<false, kTiles>(p, tab, ring, queue, active, sums, smem_u32(zeros));
+    __syncwarp();  // the warp's share of h is written
+    if (lane == 0) red_release_gpu_add(p.meeting, 1);
+    few_multiply<true, kTiles>(p, tab, ring, queue, active, sums, smem_u32(zeros));
   }
 }
 
-// An item of W13: (64 values, 16 features, gate and up, four lines); of W2: (64 values, 32 columns, four lines).  Beyond the last line or
+// An item of W13: (64 values, 32 features, gate and up, two lines); of W2: (64 values, 64 columns, two lines).  Beyond the last line or
 // feature a box holds zeros.  `tail`: a line of W2 at a time, zeros beyond the last value.
 static int few_encode(CUtensorMap* tm, const void* w, int64_t D, int64_t F, int64_t E, bool down, bool tail) {
   EncodeTiledFn enc = get_encode();
@@ -775,7 +740,7 @@ static int few_encode(CUtensorMap* tm, const void* w, int64_t D, int64_t F, int6
   const cuuint64_t dims13[5] = {64, f, 2, d / 64, e}, strides13[4] = {2 * d, 2 * f * d, 128, 4 * f * d};
   const cuuint64_t dims2[4] = {64, d, f / 64, e}, strides2[3] = {2 * f, 128, 2 * f * d};
   const cuuint64_t dims_tail[3] = {f, d, e}, strides_tail[2] = {2 * f, 2 * f * d};
-  const cuuint32_t box13[5] = {64, 16, 2, kFewLines, 1}, box2[4] = {64, kFewRows, kFewLines, 1}, box_tail[3] = {64, kFewRows, 1};
+  const cuuint32_t box13[5] = {64, kFewFeatures, 2, kFewLines, 1}, box2[4] = {64, kFewRows, kFewLines, 1}, box_tail[3] = {64, kFewRows, 1};
   const cuuint32_t step[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, tail ? 3 : down ? 4 : 5, const_cast<void*>(w),
                          tail ? dims_tail : down ? dims2 : dims13, tail ? strides_tail : down ? strides2 : strides13,
@@ -790,7 +755,7 @@ struct FewLayout {
 static FewLayout few_layout(int64_t T, int64_t F, int64_t K) {
   auto a128 = [](int64_t v) { return (v + 127) / 128 * 128; };
   const int64_t blocks = sm_count(), tiles = few_tiles(static_cast<int>(T));
-  const int64_t partial = a128(blocks * 2 * kFewRows * 8 * tiles * 4), arrived = a128(blocks * tiles * 8 * 4);
+  const int64_t partial = a128(blocks * 2 * kFewRows * 8 * tiles * 4), arrived = a128(blocks * kFewWarps * 4);
   FewLayout l;
   l.meeting = 0;
   l.arrived13 = 128;
