@@ -204,16 +204,11 @@ __device__ __forceinline__ int atom_add_acq_rel(int32_t* p, int v) {
 template <bool kDown>
 struct FewCursor {
   int strip, a, c;
-  __device__ __forceinline__ void set(int64_t item, int strips, int active, int steps) {
-    c = static_cast<int>(item % steps);
-    const int rest = static_cast<int>(item / steps);
-    if (kDown) {
-      a = rest % active;
-      strip = rest / active;
-    } else {
-      strip = rest % strips;
-      a = rest / strips;
-    }
+  __device__ __forceinline__ void set(uint32_t item, uint32_t strips, uint32_t active, uint32_t steps) {
+    const uint32_t rest = item / steps, of = kDown ? active : strips, outer = rest / of;
+    c = item - rest * steps;
+    (kDown ? a : strip) = rest - outer * of;
+    (kDown ? strip : a) = outer;
   }
   __device__ __forceinline__ void next(int strips, int active, int steps) {
     if (++c < steps) return;
@@ -245,9 +240,9 @@ struct FewWork {
         steps((inner + kFewStep - 1) / kFewStep),
         strips(kDown ? p.D / kFewRows : (p.F + kFewFeatures - 1) / kFewFeatures),  // W13: of one expert
         length(kDown ? active * steps : steps),            // items of a strip
-        split(kDown ? strips : static_cast<int64_t>(active) * strips, length, gridDim.x) {
-    const int64_t first = split.begin(blockIdx.x);
-    items = static_cast<int>(split.end(blockIdx.x) - first);
+        split(kDown ? strips : active * strips, length, gridDim.x) {
+    const uint32_t first = split.begin(blockIdx.x);
+    items = split.end(blockIdx.x) - first;
     begin.set(0, 1, 1, 1);
     tickets = !kDown && few_by_tickets(active * strips, gridDim.x);
     if (tickets)
@@ -258,7 +253,7 @@ struct FewWork {
   // The strip of a ticket; no items behind the last one.
   __device__ __forceinline__ void draw(int ticket, int active) {
     items = ticket < active * strips ? steps : 0;
-    if (items > 0) begin.set(static_cast<int64_t>(ticket) * steps, strips, active, steps);
+    if (items > 0) begin.set(ticket * steps, strips, active, steps);
   }
 };
 
@@ -551,10 +546,10 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     bool mine = true;  // to finish these rows
     if (!(whole && strip_end)) {
       // What the warps with the same rows do in every block: store their parts, arrive, and the last one finds all parts.
-      const int64_t q = kDown ? done.strip : static_cast<int64_t>(done.a) * work.strips + done.strip;  // strip of the product
+      const int q = kDown ? done.strip : done.a * work.strips + done.strip;  // strip of the product
       const int first = work.split.first_block(q), last = work.split.last_block(q);
       auto part = [&](int block) {
-        return reinterpret_cast<float4*>(phase.partial) + ((work.split.place(block, q) * kFewWarps + warp) * kTiles) * 32 + lane;
+        return reinterpret_cast<float4*>(phase.partial) + (work.split.place(block, q) * kFewWarps + warp) * kTiles * 32 + lane;
       };
       auto value = [&](int n) {  // sums: lane's row and four tokens after another
         if (!kScatter) return make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
@@ -578,6 +573,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
         float4 v[kTiles];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) v[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll(kTiles > 4 ? 2 : 4)
         for (int block = first; block <= last; ++block) {
           const float4* theirs = part(block);
 #pragma unroll
@@ -769,7 +765,11 @@ static FewLayout few_layout(int64_t T, int64_t F, int64_t K) {
 static int few_shape(int64_t T, int64_t D, int64_t F, int64_t E, int64_t K) {
   if (T <= 0 || D <= 0 || F <= 0 || E <= 0 || K <= 0) return kRcBadArg;
   if (T > kFewTokens || E > kFewExperts || K > kFewTopK) return kRcTooLarge;
-  if (D % 64 != 0 || F % 8 != 0 || D > (1 << 20) || F > (1 << 20)) return kRcUnsupportedShape;
+  if (D % 64 != 0 || F % 8 != 0) return kRcUnsupportedShape;
+  const int64_t active = T * K < E ? T * K : E, most = int64_t{1} << 30;  // items, counted in 32 bits
+  if (D > most || F > most || ceil_div64(F, kFewFeatures) * ceil_div64(D, kFewStep) > most / active ||
+      D / kFewRows * ceil_div64(F, kFewStep) > most / active)
+    return kRcTooLarge;
   return kRcOk;
 }
 
