@@ -64,24 +64,29 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _forward(x, residual, weight, eps, center, want_rstd, quantize):
     T, D = x.shape
     device = x.device
-    x = _rows(x)
-    y = torch.empty((T, D), dtype=torch.bfloat16, device=device)
+    if not x.is_contiguous():
+        x = _rows(x)
+    y = _like(x)
     total = residual_ptr = total_ptr = None
     residual_stride = residual_f32 = 0
     if residual is not None:
-        residual = _rows(residual)
-        total = torch.empty((T, D), dtype=residual.dtype, device=device)
+        if not residual.is_contiguous():
+            residual = _rows(residual)
+        total = _like(residual)
         residual_ptr, total_ptr, residual_stride = residual.data_ptr(), total.data_ptr(), residual.stride(0)
         residual_f32 = residual.dtype is torch.float32
     rstd = torch.empty(T, dtype=torch.float32, device=device) if want_rstd else None
     rows, stride = None, 0
     if quantize:
         stride = _row_bytes(D)
-        rows = (torch.zeros if stride != D + D // 32 else torch.empty)((T, stride), dtype=torch.uint8, device=device)
-    weight = weight.contiguous()
+        rows = torch.empty((T, stride), dtype=torch.uint8, device=device)
     nat.check(nat.lib.dm_add_rmsnorm_fwd(
         x.data_ptr(), x.stride(0), residual_ptr, residual_f32, residual_stride, weight.data_ptr(), weight.dtype is torch.float32,
         center, eps, T, D, total_ptr, y.data_ptr(), nat.ptr(rstd), nat.ptr(rows), stride, nat.stream_ptr()),
@@ -116,19 +121,18 @@ class _AddRmsNorm(torch.autograd.Function):
             grad_y = grad_y.contiguous()
             if grad_sum is not None:
                 grad_sum = grad_sum.contiguous()
-            gx = torch.empty((T, D), dtype=torch.bfloat16, device=device) if want_x or (want_residual and not apart) else None
+            gx = torch.empty_like(grad_y) if want_x or (want_residual and not apart) else None
             gr = torch.empty((T, D), dtype=torch.float32, device=device) if want_residual and apart else None
             gw = partial = None
             if want_weight:
-                gw = torch.empty(D, dtype=weight.dtype, device=device)
+                gw = torch.empty_like(weight)
                 partial = torch.empty((nat.lib.dm_add_rmsnorm_shares(T, D), D), dtype=torch.float32, device=device)
             if T == 0:
                 gw = gw.zero_() if want_weight else None
             else:
-                plain = weight.contiguous()
                 nat.check(nat.lib.dm_add_rmsnorm_bwd(
-                    grad_y.data_ptr(), nat.ptr(grad_sum), total.data_ptr(), apart, total.stride(0), plain.data_ptr(),
-                    plain.dtype is torch.float32, ctx.center, rstd.data_ptr(), T, D, nat.ptr(gx), nat.ptr(gr), nat.ptr(partial),
+                    grad_y.data_ptr(), nat.ptr(grad_sum), total.data_ptr(), apart, total.stride(0), weight.data_ptr(),
+                    weight.dtype is torch.float32, ctx.center, rstd.data_ptr(), T, D, nat.ptr(gx), nat.ptr(gr), nat.ptr(partial),
                     nat.ptr(gw), nat.stream_ptr()), "dm_add_rmsnorm_bwd", 2 if want_weight else 1)
         return gx if want_x else None, (gr if apart else gx) if want_residual else None, gw, None, None
 
@@ -175,6 +179,8 @@ def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: tor
             raise ValueError("quantised rows need D to be a multiple of 32 and at most 16384")
         if grads:
             raise RuntimeError("quantised rows have no gradient: call add_rms_norm(quantize=True) under torch.no_grad()")
+    if not weight_D.is_contiguous():
+        weight_D = weight_D.contiguous()
     if grads:
         got = _AddRmsNorm.apply(x_TD, residual_TD, weight_D, float(eps), float(gain_center))
         return got if residual_TD is not None else (got, x_TD)
