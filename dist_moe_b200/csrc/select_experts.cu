@@ -8,16 +8,17 @@
 // tokens, ids are -1 and scores 0, which is how the routed experts take a route that goes nowhere.  +inf logits share the softmax.
 //
 // The choice is the one of 64-bit arithmetic.  Without a bias p is monotone in l, so experts are compared by their logits.  Otherwise c
-// in 32 bits carries an error of a few units in the last place; a row in which two values that decide something lie nearer than that
-// is chosen once more in 64 bits (under one row in a hundred of normally distributed logits).
+// in 32 bits carries an error of a few units in the last place; where two values that decide something lie nearer than that, which is so
+// in under one row in a hundred of normally distributed logits, the experts in question, or for groups the whole row, are compared once
+// more in 64 bits.
 //
 // Backward, w_k = v_k / sum v, g_k = scale * grad_k:
 //   softmax            dl_i = p_i (g_i [i chosen] - sum_k p_k g_k)
 //   sigmoid            dl_k = g_k p_k (1 - p_k)
 //   softmax, normalised  dl_k = w_k (g_k - sum_j w_j g_j);   sigmoid, normalised: the same times 1 - p_k
 //
-// A warp per token: its logits sit in registers, expert 32 j + lane in register j; each of the K rounds is two warp reductions and a
-// rescan of the winning lane's registers.
+// A warp per token: its logits sit in registers, expert 32 j + lane in register j.  Each of the K rounds is two warp reductions over the
+// lanes' largest remaining values; a lane keeps its two largest, and looks through its registers again where a third is asked for.
 #include <type_traits>
 
 #include "common.cuh"
@@ -104,129 +105,202 @@ struct Top2 {
   }
 };
 
-// The choice in V arithmetic.  c(e) is the value of expert e for the comparison between groups (and between experts where `by_value`);
-// `keys` are the experts' keys in the calling warp's registers.  Returns whether two values that decide something were nearer than the
-// error of V allows; the chosen index of round k ends up in lane k.
+// The choice in V arithmetic.  `values` (shared memory of this warp, E of them) are compared between groups, `keys`, in registers, between
+// experts; whether two values are nearer than `tolerance` allows is looked at between groups and between experts where the `near_...` are
+// set.  The chosen index of round k ends up in lane k; between experts that are near one another there are more rounds than K, up to
+// the first one that stands clear of those before it.
+struct Found {
+  bool near_groups, near_experts;
+  int rounds;  // experts found, 32 at the most
+};
 template <int kPer, typename Key, typename V>
-__device__ __forceinline__ bool choose(Key (&keys)[kPer], const V* values, V tolerance, bool check, const SelectParams& p, int lane,
-                                       int& chosen) {
-  bool near = false;
+__device__ __forceinline__ Found choose(Key (&keys)[kPer], const V* values, V tolerance, bool near_groups, bool near_experts,
+                                        const SelectParams& p, int lane, int& chosen) {
+  Found found{false, false, 0};
   const V nothing = static_cast<V>(neg_inf());
   if (p.groups > 1) {
-    // lanes_per lanes look through a group; `values` is this warp's row of shared memory
     const int size = p.E / p.groups;
-    int lanes_per = 32;
-    while (32 / lanes_per < p.groups) lanes_per >>= 1;
-    const int group = lane / lanes_per, sub = lane % lanes_per;
+    int shift = 5;  // 2^shift lanes look through a group
+    while ((32 >> shift) < p.groups) --shift;
+    const int lanes_per = 1 << shift, group = lane >> shift, sub = lane & (lanes_per - 1);
     Top2<V> best{nothing, nothing};
-    if (group < p.groups)
-      for (int i = sub; i < size; i += lanes_per) best.add(values[group * size + i]);
+    if (group < p.groups) {
+      const int rounds = (size + lanes_per - 1) >> shift;
+      int k = group % rounds;  // groups start at different members: their banks differ
+      for (int i = 0; i < rounds; ++i) {
+        const int member = sub + (k << shift);
+        if (member < size) best.add(values[group * size + member]);
+        k = k + 1 == rounds ? 0 : k + 1;
+      }
+    }
     for (int d = 1; d < lanes_per; d <<= 1) {
       const V a = __shfl_xor_sync(0xffffffffu, best.first, d), b = __shfl_xor_sync(0xffffffffu, best.second, d);
       best.add(a);
       best.add(b);
     }
-    const V value = p.group_top == 2 && best.second > nothing ? best.first + best.second : best.first;
-    // rank of this lane's group: groups of larger value, or of equal value and lower index
-    int rank = 0;
-    V above = static_cast<V>(-neg_inf()), under = nothing;  // nearest values on the other side of the border
+    const bool two = p.group_top == 2 && best.second > nothing;
+    const V value = two ? best.first + best.second : best.first;
+    int rank = 0;  // groups of larger value, or of equal value and lower index
     for (int g = 0; g < p.groups; ++g) {
-      const V other = __shfl_sync(0xffffffffu, value, g * lanes_per);
+      const V other = __shfl_sync(0xffffffffu, value, g << shift);
       if (other > value || (other == value && g < group)) ++rank;
     }
     const bool keep = group < p.groups && rank < p.kept;
-    if (check && p.kept < p.groups) {
-      V span = group < p.groups && best.first > nothing ? fabs(best.first) + (p.group_top == 2 && best.second > nothing ? fabs(best.second) : V(0)) : V(0);
+    if (near_groups && p.kept < p.groups) {
+      // the smallest kept value, the largest other one, and the largest size of what was added
+      V above = keep ? value : static_cast<V>(-neg_inf()), under = keep || group >= p.groups ? nothing : value;
+      V span = group < p.groups && best.first > nothing ? fabs(best.first) + (two ? fabs(best.second) : V(0)) : V(0);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) {
-        const V other = __shfl_xor_sync(0xffffffffu, span, d);
-        span = other > span ? other : span;
-      }
-      for (int g = 0; g < p.groups; ++g) {
-        const V other = __shfl_sync(0xffffffffu, value, g * lanes_per);
-        const bool kept = __shfl_sync(0xffffffffu, keep ? 1 : 0, g * lanes_per) != 0;
-        if (kept)
-          above = other < above ? other : above;
-        else
-          under = other > under ? other : under;
+        const V a = __shfl_xor_sync(0xffffffffu, above, d), u = __shfl_xor_sync(0xffffffffu, under, d), w = __shfl_xor_sync(0xffffffffu, span, d);
+        above = a < above ? a : above;
+        under = u > under ? u : under;
+        span = w > span ? w : span;
       }
       // sums of two values each: two errors on either side.  Written so that infinities on both sides count as near.
-      near = under > nothing && !(above - under > 4 * tolerance * (1 + span));
+      found.near_groups = under > nothing && !(above - under > 4 * (tolerance + static_cast<V>(0x1p-23f) * span));
     }
-    uint32_t kept_groups = __ballot_sync(0xffffffffu, keep && sub == 0);  // bit group * lanes_per
+    const uint32_t kept_lanes = __ballot_sync(0xffffffffu, keep && sub == 0);
+    const uint32_t per_group = ((1u << 20) + size - 1) / size;  // e / size, exactly for e < 1024
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int e = 32 * j + lane;
-      if (e < p.E && !(kept_groups >> (e / size * lanes_per) & 1)) keys[j] = 0;
+      if (e < p.E && !(kept_lanes >> ((e * per_group >> 20) << shift) & 1)) keys[j] = 0;
     }
   }
-  Key mine = 0;
-  int at = 0;
-  auto rescan = [&] {
-    mine = keys[0];
-    at = 0;
+  Key mine = 0, next = 0;  // the lane's largest remaining key and the one after it
+  int at = 0, at_next = 0;
+  uint32_t gone = 0;       // registers already chosen
+  bool stale = false;      // `next` is not known
+  auto scan = [&] {
+    mine = next = 0;
+    at = at_next = 0;
 #pragma unroll
-    for (int j = 1; j < kPer; ++j)
-      if (keys[j] > mine) {
-        mine = keys[j];
+    for (int j = 0; j < kPer; ++j) {
+      const Key k = gone >> j & 1 ? 0 : keys[j];
+      if (k > mine) {
+        next = mine;
+        at_next = at;
+        mine = k;
         at = j;
+      } else if (k > next) {
+        next = k;
+        at_next = j;
       }
+    }
+    stale = false;
   };
-  rescan();
+  scan();
   chosen = -1;
   Key last = 0;
-  for (int k = 0; k < p.K + (check ? 1 : 0); ++k) {
+  auto near_last = [&](Key key) {
+    const float a = key_value(static_cast<uint32_t>(last)), b = key_value(static_cast<uint32_t>(key));
+    return !(a - b > 2.0f * (static_cast<float>(tolerance) + 0x1p-23f * fabsf(a)));
+  };
+  for (int k = 0; k < 32; ++k) {
+    if (k >= p.K && !near_experts) break;
     const Key top = warp_max_key(mine);
     if (top == 0) break;
     const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, mine == top ? static_cast<uint32_t>(32 * at + lane) : 0xffffffffu));
-    if (check && k > 0 && sizeof(Key) == 4) {
-      const float a = key_value(static_cast<uint32_t>(last)), b = key_value(static_cast<uint32_t>(top));
-      near = near || !(a - b > 2.0f * static_cast<float>(tolerance) * (1.0f + fabsf(a)));
+    if (near_experts && k > 0 && sizeof(Key) == 4) {
+      const bool near = near_last(top);
+      if (k >= p.K && !near) break;
+      found.near_experts = found.near_experts || near;
     }
+    found.rounds = k + 1;
     last = top;
-    if (k < p.K && lane == k) chosen = e;
-    if (lane == (e & 31)) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (j == (e >> 5)) keys[j] = 0;
-      rescan();
+    if (lane == k) chosen = e;
+    const bool won = lane == (e & 31);
+    if (won) gone |= 1u << at;
+    if (__any_sync(0xffffffffu, won && stale)) {
+      if (won) scan();
+    } else if (won) {
+      mine = next;
+      at = at_next;
+      next = 0;
+      stale = kPer > 2;
     }
   }
-  return near;
+  if (near_experts && found.rounds == 32) {  // and what would come after them
+    const Key top = warp_max_key(mine);
+    found.near_experts = found.near_experts || (top != 0 && near_last(top));
+  }
+  return found;
 }
 
-// The row in 64 bits: its values go through `values64`, shared memory of this warp (E doubles).
+// The sum of the softmax, in 64 bits.
+template <int kPer, typename L>
+__device__ __noinline__ double sum_again(const SelectParams& p, const L* row, float top, int lane) {
+  double z = 0.0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int e = 32 * j + lane;
+    const float l = e < p.E ? select_load(row + e) : neg_inf();
+    const bool in = l > neg_inf();
+    const double x = exp(in ? below<double>(l, top) : 0.0);
+    z += in ? x : 0.0;
+  }
+  return warp_sum(z);
+}
+
+// The order of the experts found, lane k the k-th, by their values in 64 bits: any expert that is not among them is clear of the K best.
+template <typename L>
+__device__ __noinline__ int order_again(const SelectParams& p, const L* row, float top, double z, int found, int expert, int lane) {
+  uint64_t key = 0;
+  if (lane < found) {
+    const float l = select_load(row + expert);
+    const double x = exp(p.sigmoid ? -static_cast<double>(l) : below<double>(l, top));
+    key = order_key((p.sigmoid ? 1.0 / (1.0 + x) : x / z) + static_cast<double>(p.bias[expert]));
+  }
+  int rank = 0;
+  for (int i = 0; i < found; ++i) {
+    const uint64_t other = __shfl_sync(0xffffffffu, key, i);
+    const int e = __shfl_sync(0xffffffffu, expert, i);
+    if (other > key || (other == key && e < expert)) ++rank;
+  }
+  int chosen = -1;
+  for (int k = 0; k < p.K && k < found; ++k) {
+    const uint32_t who = __ballot_sync(0xffffffffu, lane < found && rank == k);
+    const int e = __shfl_sync(0xffffffffu, expert, __ffs(static_cast<int>(who)) - 1);
+    if (lane == k) chosen = e;
+  }
+  return chosen;
+}
+
+// The row in 64 bits: its values go through `values64`, shared memory of this warp (E doubles).  No branch among a lane's values: their
+// exponentials run side by side.  (One after another they took such a row 10 us, twice the time of all others: 4096 tokens of 256 experts
+// with a bias 20 us, without one 10.)
 template <int kPer, typename L>
 __device__ __noinline__ int choose_again(const SelectParams& p, const L* row, float top, double* values64, int lane) {
-  double z = 1.0;
-  if (!p.sigmoid) {
-    z = 0.0;
-    for (int e = lane; e < p.E; e += 32) {
-      const float l = select_load(row + e);
-      if (l > neg_inf()) z += exp(below<double>(l, top));
-    }
-    z = warp_sum(z);
+  double c[kPer];
+  double z = 0.0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int e = 32 * j + lane;
+    const float l = e < p.E ? select_load(row + e) : neg_inf();
+    const bool in = l > neg_inf();
+    const double x = exp(p.sigmoid ? (in ? -static_cast<double>(l) : 0.0) : (in ? below<double>(l, top) : 0.0));
+    c[j] = in ? x : -1.0;  // -1: not to be chosen
+    z += in ? x : 0.0;
   }
+  if (!p.sigmoid) z = warp_sum(z);
   uint64_t keys[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int e = 32 * j + lane;
-    keys[j] = 0;
+    const bool in = c[j] >= 0.0;
+    double v = p.sigmoid ? 1.0 / (1.0 + (in ? c[j] : 0.0)) : (in ? c[j] : 0.0) / z;
+    if (p.bias != nullptr && e < p.E) v += static_cast<double>(p.bias[e]);
+    keys[j] = in ? order_key(v) : 0;
     if (e < p.E) {
-      const float l = select_load(row + e);
-      double c = static_cast<double>(neg_inf());
-      if (l > neg_inf()) c = (p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l))) : exp(below<double>(l, top)) / z);
-      if (p.bias != nullptr && l > neg_inf()) c += static_cast<double>(p.bias[e]);
-      keys[j] = order_key(c);
-      if (keys[j] == 0) c = static_cast<double>(neg_inf());
+      values64[e] = keys[j] != 0 ? v : static_cast<double>(neg_inf());
       // without a bias logits are compared, as in the 32-bit form
-      if (p.bias == nullptr && keys[j] != 0) keys[j] = order_key(static_cast<double>(l));
-      values64[e] = c;
+      if (p.bias == nullptr && keys[j] != 0) keys[j] = order_key(static_cast<double>(select_load(row + e)));
     }
   }
   __syncwarp();
   int chosen;
-  choose<kPer, uint64_t, double>(keys, values64, 0.0, false, p, lane, chosen);
+  choose<kPer, uint64_t, double>(keys, values64, 0.0, false, false, p, lane, chosen);
   return chosen;
 }
 
@@ -281,29 +355,17 @@ __global__ void __launch_bounds__(32 * kSelectWarps) select_experts_kernel(const
       }
     }
     if (p.groups > 1) __syncwarp();
-    // Error of c relative to 1 + |c|.  Sigmoid: exponential (1 unit in the last place, halved by p (1 - p) <= 1/4 in absolute terms),
-    // sum, quotient and the bias' addition, half a unit each: under 2^-22.  Softmax: the sum of up to 1024 terms as well, 37 roundings
-    // of half a unit: under 2^-18.
-    const float tolerance = p.sigmoid ? 0x1p-22f : 0x1p-18f;
-    bool near;
-    if (by_value) {
-      near = choose<kPer, uint32_t, float>(keys, row32, tolerance, true, p, lane, chosen);
-    } else {
-      // experts by their logits, exactly; groups by values
-      SelectParams q = p;
-      near = false;
-      if (p.groups > 1) {
-        uint32_t copy[kPer];
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) copy[j] = keys[j];
-        q.K = 0;  // the groups' border alone
-        near = choose<kPer, uint32_t, float>(copy, row32, tolerance, true, q, lane, chosen);
-      }
-      choose<kPer, uint32_t, float>(keys, row32, tolerance, false, p, lane, chosen);
-    }
-    if (values && near) {
+    // Error of p, in units of 2^-24.  Sigmoid: exponential 4 times p (1 - p), sum and quotient 1 each times p: under 3.  Softmax, relative
+    // to p <= 1 / z: rounding of the exponent d e^-d <= 0.4, exponential 4, a sum of up to 1024 such terms in 37 roundings, quotient 1:
+    // under 64.  The bias' addition is half a unit of c in the last place.
+    const float tolerance = p.sigmoid ? 0x1p-22f : 0x1p-18f / z;
+    // without a bias experts go by their logits, exactly
+    const Found found = choose<kPer, uint32_t, float>(keys, row32, tolerance, values, by_value, p, lane, chosen);
+    if (found.near_groups || (found.near_experts && found.rounds == 32)) {
       __syncwarp();
       chosen = choose_again<kPer, L>(p, row, top, row64, lane);
+    } else if (found.near_experts) {
+      chosen = order_again<L>(p, row, top, p.sigmoid ? 1.0 : sum_again<kPer, L>(p, row, top, lane), found.rounds, chosen, lane);
     }
     // lane k: the score of the k-th
     const bool have = lane < p.K && chosen >= 0;

@@ -134,18 +134,22 @@ def test_equal_values_go_to_the_lowest_index():
     _check(_logits(50, 64, torch.bfloat16, spread=0.02), 8, bias_E=torch.zeros(64, device=DEV))  # many equal logits
 
 
+# few experts near one another; more than a warp has lanes; as many chosen as a warp has lanes
+@pytest.mark.parametrize("E,K", [(24, 6), (48, 6), (66, 32)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
-def test_values_that_32_bits_cannot_tell_apart(score):
-    """Choices that hang on differences far below an fp32 unit of c: the row is chosen in 64 bits."""
+def test_values_that_32_bits_cannot_tell_apart(score, E, K):
+    """Choices that hang on differences far below an fp32 unit of c: they are made in 64 bits."""
     g = torch.Generator().manual_seed(1)
-    T, E = 64, 48
+    T = 64
     logits = torch.randn(T, 1, generator=g).expand(T, E).clone()
     logits += torch.randint(-3, 4, (T, E), generator=g) * 2.0 ** -22  # neighbours in fp32
     bias = torch.randint(0, 2, (E,), generator=g) * 2.0 ** -26
     logits, bias = logits.to(DEV), bias.to(DEV)
-    _check(logits, 6, score=score, bias_E=bias)
-    _check(logits, 6, score=score, bias_E=bias, num_groups=6, num_kept_groups=3)
-    _check(logits, 6, score=score, num_groups=6, num_kept_groups=3)
+    _check(logits, K, score=score, bias_E=bias)
+    _check(logits, K, score=score, bias_E=bias, num_groups=6, num_kept_groups=3)
+    _check(logits, K, score=score, num_groups=6, num_kept_groups=3)
+    logits[:, ::5] += 1.0  # some stand clear
+    _check(logits, K, score=score, bias_E=bias)
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
