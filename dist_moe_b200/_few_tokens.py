@@ -7,16 +7,17 @@ import torch
 from . import _native as nat
 
 MAX_TOKENS = 64  # DM_FEW_TOKENS_MAX
+COUNTER_BYTES = 8192  # DM_FEW_TOKENS_COUNTER_BYTES
 
 
 def workspace(state) -> torch.Tensor | None:
-    """What a context keeps for calls of few tokens, zeroed once: None where they are not offered."""
+    """What a context keeps for calls of few tokens, None where they are not offered.  The context clears its counters."""
     cfg = state.config
     if state.ep != 1 or state.block_scaled:
         return None
     nbytes = nat.lib.dm_few_tokens_workspace_bytes(min(MAX_TOKENS, cfg.max_num_local_input_tokens), cfg.hidden_dim,
                                                    cfg.intermediate_dim, cfg.num_experts, cfg.top_k)
-    return torch.zeros(nbytes, dtype=torch.uint8, device=state.device) if nbytes > 0 else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=state.device) if nbytes > 0 else None
 
 
 def run(x, ids, scores, w13, w2, state) -> torch.Tensor:

@@ -162,7 +162,7 @@ class ContextState:
         gathered that are not."""
         self.gather_flags.zero_()
         if self.few_workspace is not None:
-            self.few_workspace.zero_()
+            self.few_workspace[:_few_tokens.COUNTER_BYTES].zero_()
 
     def select_slot(self, slot: int, num_layers: int) -> None:
         if self.num_slots == 0:

@@ -695,6 +695,9 @@ def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tens
     w13_EFD, w2_EDF = _reshape_weights(w13_weight, w2_weight, state.e_local, context.config)
     if isinstance(x_TD, QuantizedRows):
         raise TypeError("x_TD must use torch.bfloat16")
+    # a few rows in another layout are copied, weights are not
+    x_TD, topk_expert_ids_TK, topk_scores_TK = (t if t.is_contiguous() else t.contiguous()
+                                                for t in (x_TD, topk_expert_ids_TK, topk_scores_TK))
     _validate_inputs(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, context, prepared=False)
     if x_TD.device != state.device:
         raise ValueError(f"x_TD is on {x_TD.device} but the context was created on {state.device}")

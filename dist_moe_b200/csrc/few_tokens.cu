@@ -22,6 +22,7 @@
 // then read 16 bytes a lane along the inner dimension as they lie in shared memory, its order inside 32 values being the same for both
 // (lane t of a row holds values 8 t .. 8 t + 7, in two instructions), and a gate value meets its up value in the same lane.  Row g of
 // the instruction is row few_row(g) of the warp's rows, which keeps the reads of the 128-byte swizzle free of bank conflicts.
+#include <algorithm>
 #include <type_traits>
 
 #include "few_split.cuh"
@@ -45,8 +46,8 @@ constexpr int kFewRowPitch = kFewStep * 2 + 64;    // rows of x or h: eight of t
 constexpr int kFewMaxDepth = 13;
 constexpr int kFewQueue = 4;                       // tickets on their way from the weights' warp to the others
 __host__ __device__ constexpr int few_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8; }
-// W2 of more than one tile: a sum for every row and token.
-__host__ __device__ constexpr int few_sum_bytes(int T, int tiles) { return tiles > 1 ? (kFewRows * (T | 1) * 4 + 15) / 16 * 16 : 0; }
+// W2: a sum for every row and token.
+__host__ __device__ constexpr int few_sum_bytes(int T) { return (kFewRows * (T | 1) * 4 + 15) / 16 * 16; }
 constexpr uint64_t kFewWaitNs = 2000000000ull;
 
 struct FewPhase {
@@ -226,7 +227,10 @@ struct FewCursor {
 };
 
 // Whole strips by tickets, where the last round of them is full enough.
-__device__ __forceinline__ bool few_by_tickets(int strips, int blocks) { return 5 * strips >= 4 * blocks * ((strips + blocks - 1) / blocks); }
+__device__ __forceinline__ bool few_by_tickets(uint32_t strips, uint32_t blocks) {
+  const uint64_t rounds = (strips + blocks - 1) / blocks;
+  return 5ull * strips >= 4 * rounds * blocks;
+}
 
 // What the warps of a block know of one of the two products.
 template <bool kDown>
@@ -386,12 +390,11 @@ __device__ __noinline__ void few_wait_on(uint64_t* bar, uint32_t parity, int* ab
 }
 
 // The warps that multiply.  kTiles: tiles of eight columns that the accumulators hold.  Columns are an expert's tokens, next to one
-// another; W2, which sums over the experts, adds them to sums by token in shared memory at the end of each expert's items.  Up to eight
-// tokens are one tile anyhow: there W2's columns are the tokens themselves.  (With them as columns at every size, 32 and 64 tokens of the
-// layer above took 230 and 370 us where 215 and 285 were reached.)
+// another; W2, which sums over the experts, adds them to sums by token in shared memory at the end of each expert's items.  (With all tokens
+// as W2's columns, zero where they are not the expert's, 32 and 64 tokens of the layer above took 230 and 370 us where 215 and 285 were
+// reached, and a weight that is not finite reached every token.)
 template <bool kDown, int kTiles>
-__device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, float* all_sums,
-                                             uint32_t zeros) {
+__device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, float* all_sums) {
   FewWork<kDown> work(p, active);
   const FewPhase& phase = p.phase[kDown];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -402,7 +405,6 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
   const int r0 = warp * (kDown ? 16 : 8) + rho;
   const uint32_t at_w = smem_u32(ring.base) + r0 * 128 + ((quad ^ rho) << 4);
   const uint32_t at_b = smem_u32(ring.base) + kFewWeightBytes + quad * 16;
-  const uint32_t none = zeros + quad * 16;
   const uint32_t full0 = smem_u32(ring.full), empty0 = smem_u32(ring.empty);
   int place = ring.place;
   uint32_t round = ring.round, here = place * ring.place_bytes;
@@ -413,7 +415,6 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
   };
-  constexpr bool kScatter = kDown && kTiles > 1, kByToken = kDown && kTiles == 1;
   const int pitch = p.T | 1;
   float* sums = all_sums + warp * 16 * pitch;  // of this warp's rows, by token
   auto clear_sums = [&] {
@@ -421,18 +422,12 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     __syncwarp();
   };
   int tiles = 0;
-  int from[kTiles];  // offset of the column's row in a place, -1 for a token that is not the expert's
-  auto columns = [&](int a) {
+  int from[kTiles];  // offset of the column's row in a place
+  auto columns = [&](int a) {  // columns beyond the last token repeat it, and are not kept
     const int count = tab.base[a + 1] - tab.base[a];
-    if (kByToken) {
-      const uint64_t tokens = tab.tokens[tab.expert[a]];
-      tiles = 1;
-      from[0] = (tokens >> g) & 1 ? __popcll(tokens & ((1ull << g) - 1)) * kFewRowPitch : -1;
-    } else {  // columns beyond the last token repeat it, and are not kept
-      tiles = (count + 7) >> 3;
+    tiles = (count + 7) >> 3;
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) from[n] = min(8 * n + g, count - 1) * kFewRowPitch;
-    }
+    for (int n = 0; n < kTiles; ++n) from[n] = min(8 * n + g, count - 1) * kFewRowPitch;
   };
   // A line's operands.
   struct Operands {
@@ -447,7 +442,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       const uint32_t aw = (at_w + here + line * kFewLineBytes) ^ (h << 6);
       x.lo[h] = lds16(aw);
       x.hi[h] = lds16(aw + up * 128);
-      x.b[h] = lds16((kByToken && from[0] < 0 ? none : at_b + here + from[0]) + line * 128 + h * 64);
+      x.b[h] = lds16(at_b + here + from[0] + line * 128 + h * 64);
     }
   };
   auto multiply = [&](float (&to)[4], const Operands& x, const uint4& b, int h) {
@@ -507,7 +502,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     }
   };
   clear();
-  if (kScatter) clear_sums();
+  if (kDown) clear_sums();
   FewCursor<kDown> at = work.begin;
   bool whole = at.c == 0 && (!kDown || at.a == 0);  // the strip from its first item on
   for (int left = work.items; left > 0;) {
@@ -523,7 +518,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     const int base = tab.base[at.a], pairs = tab.base[at.a + 1] - base;
     at.c += n_items - 1;
     at.next(work.strips, active, work.steps);
-    if (kScatter) {
+    if (kDown) {
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
         if (n >= tiles) break;
@@ -552,12 +547,12 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
         return reinterpret_cast<float4*>(phase.partial) + (work.split.place(block, q) * kFewWarps + warp) * kTiles * 32 + lane;
       };
       auto value = [&](int n) {  // sums: lane's row and four tokens after another
-        if (!kScatter) return make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+        if (!kDown) return make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
         const float* of = sums + (lane & 15) * pitch;
         const int t = 8 * n + 4 * (lane >> 4);
         return make_float4(t < p.T ? of[t] : 0.f, t + 1 < p.T ? of[t + 1] : 0.f, t + 2 < p.T ? of[t + 2] : 0.f, t + 3 < p.T ? of[t + 3] : 0.f);
       };
-      const int used = kScatter ? (p.T + 7) >> 3 : tiles;
+      const int used = kDown ? (p.T + 7) >> 3 : tiles;
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
         if (n < used) __stcg(part(blockIdx.x) + n * 32, value(n));
@@ -585,7 +580,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
         }
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
-          if (!kScatter) {
+          if (!kDown) {
             acc[n][0] = v[n].x, acc[n][1] = v[n].y, acc[n][2] = v[n].z, acc[n][3] = v[n].w;
           } else if (n < used) {
             float* of = sums + (lane & 15) * pitch;
@@ -600,17 +595,9 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       }
     }
     if (mine) {
-      if (kScatter) {
+      if (kDown) {
         __nv_bfloat16* to = p.out + done.strip * kFewRows + warp * 16 + (lane & 15);
         for (int t = lane >> 4; t < p.T; t += 2) to[static_cast<int64_t>(t) * p.D] = __float2bfloat16_rn(sums[(lane & 15) * pitch + t]);
-      } else if (kByToken) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (2 * quad + j < p.T) {
-            __nv_bfloat16* to = p.out + static_cast<int64_t>(2 * quad + j) * p.D + done.strip * kFewRows + r0;
-            to[0] = __float2bfloat16_rn(acc[0][j]);
-            to[up] = __float2bfloat16_rn(acc[0][2 + j]);
-          }
       } else if (done.strip * kFewFeatures + r0 < p.F) {
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
@@ -627,7 +614,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
         }
       }
     }
-    if (kScatter) {
+    if (kDown) {
       __syncwarp();
       clear_sums();
     }
@@ -650,9 +637,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
   uint8_t* smem = few_smem_raw + (-smem_u32(few_smem_raw) & 1023u);  // an offset: what lies there stays known as shared memory
   __shared__ uint64_t full[kFewMaxDepth], empty[kFewMaxDepth], queue_full[kFewQueue], queue_empty[kFewQueue];
   __shared__ int s_found[2], s_ticket[kFewQueue], abort_flag;
-  __shared__ __align__(16) uint8_t zeros[kFewStep * 2 + 16];  // a row for the columns that an expert has none for
   float* sums = reinterpret_cast<float*>(smem + ring_bytes);
-  const FewTables tab(smem + ring_bytes + few_sum_bytes(p.T, kTiles), p.T, p.E, p.K);
+  const FewTables tab(smem + ring_bytes + few_sum_bytes(p.T), p.T, p.E, p.K);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == kFewWarps) {
     if (lane < kFewMaxDepth) {
@@ -666,12 +652,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
     if (lane == 0) {
       abort_flag = 0;
       tma_prefetch_desc(&p.phase[0].items);
-      tma_prefetch_desc(&p.phase[1].items);
+      if (p.F >= 64) tma_prefetch_desc(&p.phase[1].items);
     }
     mbar_fence_init();
     fence_proxy_async_smem();
   }
-  if (threadIdx.x < sizeof(zeros) / 4) reinterpret_cast<uint32_t*>(zeros)[threadIdx.x] = 0;
   int most;
   const int active = few_tables(p, tab, s_found, blockIdx.x == 0, most);
   if (active == 0) {  // nothing is routed anywhere: all blocks see it
@@ -720,10 +705,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
       tab.share[i] = share;
     }
     multipliers_meet();  // shares are there
-    few_multiply<false, kTiles>(p, tab, ring, queue, active, sums, smem_u32(zeros));
+    few_multiply<false, kTiles>(p, tab, ring, queue, active, sums);
     __syncwarp();  // the warp's share of h is written
     if (lane == 0) red_release_gpu_add(p.meeting, 1);
-    few_multiply<true, kTiles>(p, tab, ring, queue, active, sums, smem_u32(zeros));
+    few_multiply<true, kTiles>(p, tab, ring, queue, active, sums);
   }
 }
 
@@ -756,7 +741,7 @@ static FewLayout few_layout(int64_t T, int64_t F, int64_t K) {
   l.meeting = 0;
   l.arrived13 = 128;
   l.arrived2 = l.arrived13 + arrived;
-  l.partial13 = l.arrived2 + arrived;
+  l.partial13 = std::max<int64_t>(l.arrived2 + arrived, DM_FEW_TOKENS_COUNTER_BYTES);
   l.partial2 = l.partial13 + partial;
   l.h = l.partial2 + partial;
   l.total = l.h + a128(T * K * F * 2);
@@ -765,7 +750,7 @@ static FewLayout few_layout(int64_t T, int64_t F, int64_t K) {
 static int few_shape(int64_t T, int64_t D, int64_t F, int64_t E, int64_t K) {
   if (T <= 0 || D <= 0 || F <= 0 || E <= 0 || K <= 0) return kRcBadArg;
   if (T > kFewTokens || E > kFewExperts || K > kFewTopK) return kRcTooLarge;
-  if (D % 64 != 0 || F % 8 != 0) return kRcUnsupportedShape;
+  if (D % 64 != 0 || F % 8 != 0 || 128 + 2 * (sm_count() * kFewWarps * 4 + 127) > DM_FEW_TOKENS_COUNTER_BYTES) return kRcUnsupportedShape;
   const int64_t active = T * K < E ? T * K : E, most = int64_t{1} << 30;  // items, counted in 32 bits
   if (D > most || F > most || ceil_div64(F, kFewFeatures) * ceil_div64(D, kFewStep) > most / active ||
       D / kFewRows * ceil_div64(F, kFewStep) > most / active)
@@ -817,7 +802,7 @@ extern "C" int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, 
   auto run = [&](auto tiles_tag) {
     constexpr auto kernel = few_tokens_kernel<decltype(tiles_tag)::value>;
     constexpr int most = 226 * 1024;
-    const int red = few_sum_bytes(p.T, decltype(tiles_tag)::value), tables = FewTables::bytes(p.T, p.E, p.K);
+    const int red = few_sum_bytes(p.T), tables = FewTables::bytes(p.T, p.E, p.K);
     const int ring = (most - 1024 - red - tables) / 1024 * 1024;
     static PerDeviceOnce attr_set;
     const int arc = once_per_device(attr_set, [] {

@@ -147,6 +147,23 @@ def test_nonfinite_tokens_stay_with_themselves():
     ctx.close()
 
 
+@pytest.mark.parametrize("T", [2, 8, 20])
+@pytest.mark.parametrize("which", ["w13", "w2"])
+def test_nonfinite_weights_reach_their_own_tokens_alone(T, which):
+    D, F, E, K = 128, 72, 6, 2
+    x, ids, scores, w13, w2 = _case(T, D, F, E, K)
+    ids[:] = torch.tensor([0, 1], device=DEV, dtype=ids.dtype)
+    ids[1] = torch.tensor([4, 2], device=DEV, dtype=ids.dtype)
+    ctx = _context(T, D, F, E, K)
+    clean = dm.routed_experts_few_tokens(x, ids, scores, w13, w2, ctx)
+    w = (w13 if which == "w13" else w2).clone()
+    w[4] = float("inf")
+    got = dm.routed_experts_few_tokens(x, ids, scores, w if which == "w13" else w13, w2 if which == "w13" else w, ctx)
+    keep = torch.arange(T) != 1
+    assert not got[1].isfinite().any() and torch.equal(got[keep], clean[keep])
+    ctx.close()
+
+
 def test_fewer_tokens_than_the_context_holds_and_calls_in_turn():
     D, F, E, K = 256, 264, 16, 4
     ctx = _context(500, D, F, E, K)
@@ -159,6 +176,10 @@ def test_fewer_tokens_than_the_context_holds_and_calls_in_turn():
         assert torch.equal(dm.routed_experts_few_tokens(*case, training), dm.routed_experts_few_tokens(*case, ctx))
     small = _context(500, D, F, E, K, num_sms=3)
     _check(dm.routed_experts_few_tokens(*case, small), case)
+    wide = [torch.cat([t, t], 1)[:, :t.shape[1]] for t in case[:3]]  # slices are copied
+    assert torch.equal(dm.routed_experts_few_tokens(*wide, *case[3:], ctx), dm.routed_experts_few_tokens(*case, ctx))
+    with pytest.raises(ValueError, match="contiguous"):
+        dm.routed_experts_few_tokens(*case[:4], case[4].transpose(1, 2).contiguous().transpose(1, 2), ctx)
     w4 = case[3].view(E, 2, F, D)
     assert torch.equal(dm.routed_experts_few_tokens(*case[:3], w4, case[4], ctx), dm.routed_experts_few_tokens(*case, ctx))
     for c in (ctx, training, small):
