@@ -72,27 +72,27 @@ struct FewParams {
 
 // Which experts are hit, by which tokens: built by every block.
 struct FewTables {
-  uint64_t* tokens;  // [E] bit t: token t
-  float* score;      // [T K]
-  float* share;      // [pairs] c[t, e]
-  int16_t* expert;   // [active]
-  int16_t* base;     // [active + 1] first pair
-  int16_t* owner;    // [pairs] active expert
-  int16_t* id;       // [T K]
-  uint8_t* token;    // [pairs]
+  uint2* tokens;    // [E] bit t: token t
+  float* score;     // [T K]
+  float* share;     // [pairs] c[t, e]
+  int16_t* expert;  // [active]
+  int16_t* base;    // [active + 1] first pair
+  int16_t* first;   // [E] the same by expert
+  int16_t* id;      // [T K]
+  uint8_t* token;   // [pairs]
   __device__ __forceinline__ FewTables(uint8_t* at, int T, int E, int K) {
     const int active = T * K < E ? T * K : E;
-    tokens = reinterpret_cast<uint64_t*>(at);
+    tokens = reinterpret_cast<uint2*>(at);
     score = reinterpret_cast<float*>(tokens + E);
     share = score + T * K;
     expert = reinterpret_cast<int16_t*>(share + T * K);
     base = expert + active;
-    owner = base + active + 1;
-    id = owner + T * K;
+    first = base + active + 1;
+    id = first + E;
     token = reinterpret_cast<uint8_t*>(id + T * K);
   }
   static __host__ __device__ constexpr int bytes(int T, int E, int K) {
-    return (8 * E + 13 * T * K + 4 * (T * K < E ? T * K : E) + 2 + 15) / 16 * 16;
+    return (10 * E + 11 * T * K + 4 * (T * K < E ? T * K : E) + 2 + 15) / 16 * 16;
   }
 };
 
@@ -105,27 +105,43 @@ __device__ __forceinline__ int few_id(const FewParams& p, int i) {
   return v >= 0 && v < p.E ? v : v == -1 ? -1 : -2;
 }
 
-// Returns the number of experts that are hit; `most` is the largest number of tokens of one.
+__device__ __forceinline__ float few_score(const FewParams& p, int i) {
+  return p.scores_are_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.scores)[i]) : static_cast<const float*>(p.scores)[i];
+}
+
+// All warps: the experts that are hit and their pairs' places.  Returns their number; `most` is the largest number of tokens of one.
 __device__ __forceinline__ int few_tables(const FewParams& p, const FewTables& s, int (&s_found)[2], bool report, int& most) {
-  for (int e = threadIdx.x; e < p.E; e += kFewThreads) s.tokens[e] = 0;
+  const int routes = p.T * p.K;
+  int i = threadIdx.x, id = -1;
+  float score = 0.f;
+  if (i < routes) {  // on their way while the masks are cleared
+    id = few_id(p, i);
+    score = few_score(p, i);
+  }
+  for (int e = threadIdx.x; e < p.E; e += kFewThreads) s.tokens[e] = make_uint2(0, 0);
   __syncthreads();
-  for (int i = threadIdx.x; i < p.T * p.K; i += kFewThreads) {
-    s.score[i] = p.scores_are_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.scores)[i]) : static_cast<const float*>(p.scores)[i];
-    const int id = few_id(p, i);
+  while (i < routes) {
+    const int t = i / p.K;
+    s.score[i] = score;
     s.id[i] = static_cast<int16_t>(id);
     if (id >= 0)
-      atomicOr(reinterpret_cast<unsigned long long*>(&s.tokens[id]), 1ull << (i / p.K));
+      atomicOr(t < 32 ? &s.tokens[id].x : &s.tokens[id].y, 1u << (t & 31));
     else if (id == -2 && report)
       set_status(p.status, kInvalidExpertId, i);
+    i += kFewThreads;
+    if (i < routes) {
+      id = few_id(p, i);
+      score = few_score(p, i);
+    }
   }
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int active = 0, pairs = 0, largest = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const uint64_t tokens = e0 + lane < p.E ? s.tokens[e0 + lane] : 0;
-      const uint32_t hit = __ballot_sync(0xffffffffu, tokens != 0);
-      const int own = __popcll(tokens);
+      const uint2 tokens = e0 + lane < p.E ? s.tokens[e0 + lane] : make_uint2(0, 0);
+      const int own = __popc(tokens.x) + __popc(tokens.y);
+      const uint32_t hit = __ballot_sync(0xffffffffu, own != 0);
       int before = own;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -133,15 +149,10 @@ __device__ __forceinline__ int few_tables(const FewParams& p, const FewTables& s
         if (lane >= d) before += v;
       }
       const int total = __shfl_sync(0xffffffffu, before, 31);
-      if (tokens != 0) {
-        const int at = active + __popc(hit & ((1u << lane) - 1));
-        int n = pairs + before - own;
+      if (own != 0) {
+        const int at = active + __popc(hit & ((1u << lane) - 1)), n = pairs + before - own;
         s.expert[at] = static_cast<int16_t>(e0 + lane);
-        s.base[at] = static_cast<int16_t>(n);
-        for (uint64_t left = tokens; left != 0; left &= left - 1, ++n) {
-          s.token[n] = static_cast<uint8_t>(__ffsll(static_cast<long long>(left)) - 1);
-          s.owner[n] = static_cast<int16_t>(at);
-        }
+        s.base[at] = s.first[e0 + lane] = static_cast<int16_t>(n);
       }
       active += __popc(hit);
       pairs += total;
@@ -157,6 +168,27 @@ __device__ __forceinline__ int few_tables(const FewParams& p, const FewTables& s
   __syncthreads();
   most = s_found[1];
   return s_found[0];
+}
+
+// The warps that need them, thread `rank` of `ranks`: the pairs' tokens and shares, a pair by the first of its routes.
+__device__ __forceinline__ void few_pairs(const FewParams& p, const FewTables& s, int rank, int ranks) {
+  for (int i = rank; i < p.T * p.K; i += ranks) {
+    const int id = s.id[i], t = i / p.K, row = t * p.K;
+    if (id < 0) continue;
+    bool again = false;
+    float share = 0.f;
+    for (int j = row; j < row + p.K; ++j) {
+      const bool same = s.id[j] == id;
+      again = again || (same && j < i);
+      if (same) share += s.score[j];
+    }
+    if (again) continue;
+    const uint2 tokens = s.tokens[id];
+    const uint32_t below = (1u << (t & 31)) - 1;
+    const int pair = s.first[id] + (t < 32 ? __popc(tokens.x & below) : __popc(tokens.x) + __popc(tokens.y & below));
+    s.token[pair] = static_cast<uint8_t>(t);
+    s.share[pair] = share;
+  }
 }
 
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
@@ -191,7 +223,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool i
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void multipliers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory"); }
 // Row g of the instruction: neighbouring ones differ in the swizzle's third bit.
 __device__ __forceinline__ constexpr int few_row(int g) { return (g >> 1) | ((g & 1) << 2); }
 __device__ __forceinline__ int atom_add_acq_rel(int32_t* p, int v) {
@@ -678,7 +709,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
       if (!ok) set_status(p.status, kPipelineTimeout, 6, blockIdx.x);
       settle_ring(full, ring.depth, ring_stop(ring.place, ring.round), globaltimer_ns() + (ok ? kFewWaitNs : kSettleNs));
     }
-  } else if (warp == kFewWarps + 1) {
+    return;
+  }
+  constexpr int kOthers = 32 * (kFewWarps + 1);
+  few_pairs(p, tab, warp == kFewWarps + 1 ? 32 * kFewWarps + lane : threadIdx.x, kOthers);
+  asm volatile("bar.sync 1, %0;" ::"n"(kOthers) : "memory");
+  if (warp == kFewWarps + 1) {
     bool ok = few_load_rows<false>(p, tab, ring, queue, active, lane);
     if (ok) {  // until h is there
       const uint64_t t0 = globaltimer_ns();
@@ -697,14 +733,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_tokens_kernel(const __grid
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
-    for (int i = threadIdx.x; i < tab.base[active]; i += 32 * kFewWarps) {
-      const int t = tab.token[i], e = tab.expert[tab.owner[i]];
-      float share = 0.f;
-      for (int k = 0; k < p.K; ++k)
-        if (tab.id[t * p.K + k] == e) share += tab.score[t * p.K + k];
-      tab.share[i] = share;
-    }
-    multipliers_meet();  // shares are there
     few_multiply<false, kTiles>(p, tab, ring, queue, active, sums);
     __syncwarp();  // the warp's share of h is written
     if (lane == 0) red_release_gpu_add(p.meeting, 1);
