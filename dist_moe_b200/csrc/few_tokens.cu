@@ -46,7 +46,7 @@ constexpr int kFewRowPitch = kFewStep * 2 + 64;    // rows of x or h: eight of t
 constexpr int kFewMaxDepth = 13;
 constexpr int kFewQueue = 4;                       // tickets on their way from the weights' warp to the others
 __host__ __device__ constexpr int few_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8; }
-// W2: a sum for every row and token.
+// A sum for every row and token.
 __host__ __device__ constexpr int few_sum_bytes(int T) { return (kFewRows * (T | 1) * 4 + 15) / 16 * 16; }
 constexpr uint64_t kFewWaitNs = 2000000000ull;
 
@@ -421,7 +421,8 @@ __device__ __noinline__ void few_wait_on(uint64_t* bar, uint32_t parity, int* ab
 }
 
 // The warps that multiply.  kTiles: tiles of eight columns that the accumulators hold.  Columns are an expert's tokens, next to one
-// another; W2, which sums over the experts, adds them to sums by token in shared memory at the end of each expert's items.  (With all tokens
+// another.  At the end of a strip the sums go through shared memory (the code for every tile's activation or partial sums in a row made
+// the launch slower: what the warps run has to stay small); W2, which sums over the experts, adds them there by token after each expert.  (With all tokens
 // as W2's columns, zero where they are not the expert's, 32 and 64 tokens of the layer above took 230 and 370 us where 215 and 285 were
 // reached, and a weight that is not finite reached every token.)
 template <bool kDown, int kTiles>
@@ -512,23 +513,28 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     for (int j = 0; j < 4; ++j) acc[0][j] += odd[j];
   };
   auto run = [&](int n_items, int lines) {
+    Operands x, y;
+    auto line_of = [&](const Operands& of, int line) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 b = of.b[h];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          if (n >= tiles) break;
+          uint4 next = b;
+          if (n + 1 < kTiles && n + 1 < tiles) next = lds16(at_b + here + from[n + 1 < kTiles ? n + 1 : n] + line * 128 + h * 64);
+          multiply(acc[n], of, b, h);
+          b = next;
+        }
+      }
+    };
 #pragma unroll 1
     for (int i = 0; i < n_items; ++i, lines -= kFewLines) {
       wait();
-#pragma unroll 1
-      for (int line = 0; line < min(lines, kFewLines); ++line) {
-        Operands x;
-        fetch(x, line);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          multiply(acc[0], x, x.b[h], h);
-#pragma unroll
-          for (int n = 1; n < kTiles; ++n) {
-            if (n >= tiles) break;
-            multiply(acc[n], x, lds16(at_b + here + from[n] + line * 128 + h * 64), h);
-          }
-        }
-      }
+      fetch(x, 0);
+      if (lines > 1) fetch(y, 1);
+      line_of(x, 0);
+      if (lines > 1) line_of(y, 1);
       leave();
     }
   };
@@ -549,7 +555,9 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     const int base = tab.base[at.a], pairs = tab.base[at.a + 1] - base;
     at.c += n_items - 1;
     at.next(work.strips, active, work.steps);
-    if (kDown) {
+    const bool strip_end = kDown ? at.strip != done.strip : at.c == 0;
+    const bool ends = strip_end || left == 0;
+    if (kDown || ends) {
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
         if (n >= tiles) break;
@@ -557,18 +565,18 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
         for (int j = 0; j < 2; ++j) {
           const int col = 8 * n + 2 * quad + j;
           if (col < pairs) {
-            float* to = sums + tab.token[base + col] + rho * pitch;
-            to[0] += acc[n][j];
-            to[up * pitch] += acc[n][2 + j];
+            float* to = sums + (kDown ? tab.token[base + col] : col) + rho * pitch;
+            to[0] = kDown ? to[0] + acc[n][j] : acc[n][j];
+            to[8 * pitch] = kDown ? to[8 * pitch] + acc[n][2 + j] : acc[n][2 + j];
           }
         }
       }
       __syncwarp();
       clear();
     }
-    const bool strip_end = kDown ? at.strip != done.strip : at.c == 0;
-    if (!strip_end && left > 0) continue;
+    if (!ends) continue;
     // ---- the end of the strip, or of the block's part of it ------------------------------------------------------------------
+    const int cols = kDown ? p.T : pairs;
     bool mine = true;  // to finish these rows
     if (!(whole && strip_end)) {
       // What the warps with the same rows do in every block: store their parts, arrive, and the last one finds all parts.
@@ -577,16 +585,15 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       auto part = [&](int block) {
         return reinterpret_cast<float4*>(phase.partial) + (work.split.place(block, q) * kFewWarps + warp) * kTiles * 32 + lane;
       };
-      auto value = [&](int n) {  // sums: lane's row and four tokens after another
-        if (!kDown) return make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-        const float* of = sums + (lane & 15) * pitch;
-        const int t = 8 * n + 4 * (lane >> 4);
-        return make_float4(t < p.T ? of[t] : 0.f, t + 1 < p.T ? of[t + 1] : 0.f, t + 2 < p.T ? of[t + 2] : 0.f, t + 3 < p.T ? of[t + 3] : 0.f);
-      };
-      const int used = kDown ? (p.T + 7) >> 3 : tiles;
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-        if (n < used) __stcg(part(blockIdx.x) + n * 32, value(n));
+      // A lane's pieces: its row, four columns after another.
+      float* row = sums + (lane & 15) * pitch;
+      const int col0 = 4 * (lane >> 4), used = (cols + 7) >> 3;
+#pragma unroll 1
+      for (int n = 0; n < used; ++n) {
+        const int c = 8 * n + col0;
+        __stcg(part(blockIdx.x) + n * 32, make_float4(c < cols ? row[c] : 0.f, c + 1 < cols ? row[c + 1] : 0.f, c + 2 < cols ? row[c + 2] : 0.f,
+                                                     c + 3 < cols ? row[c + 3] : 0.f));
+      }
       __syncwarp();
       int before = 0;
       if (lane == 0) {
@@ -596,30 +603,29 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       }
       mine = __shfl_sync(0xffffffffu, before, 0) == last - first;
       if (mine) {
-        float4 v[kTiles];
+#pragma unroll 1
+        for (int n0 = 0; n0 < used; n0 += 4) {  // four pieces of several blocks on their way at a time
+          constexpr int kN = kTiles < 4 ? kTiles : 4;
+          float4 v[kN];
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n) v[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll(kTiles > 4 ? 2 : 4)
-        for (int block = first; block <= last; ++block) {
-          const float4* theirs = part(block);
+          for (int i = 0; i < kN; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll(kN > 2 ? 2 : 4)
+          for (int block = first; block <= last; ++block) {
+            const float4* theirs = part(block) + n0 * 32;
 #pragma unroll
-          for (int n = 0; n < kTiles; ++n)
-            if (n < used) {
-              const float4 add = __ldcg(theirs + n * 32);
-              v[n].x += add.x, v[n].y += add.y, v[n].z += add.z, v[n].w += add.w;
-            }
-        }
+            for (int i = 0; i < kN; ++i)
+              if (n0 + i < used) {
+                const float4 add = __ldcg(theirs + i * 32);
+                v[i].x += add.x, v[i].y += add.y, v[i].z += add.z, v[i].w += add.w;
+              }
+          }
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          if (!kDown) {
-            acc[n][0] = v[n].x, acc[n][1] = v[n].y, acc[n][2] = v[n].z, acc[n][3] = v[n].w;
-          } else if (n < used) {
-            float* of = sums + (lane & 15) * pitch;
-            const int t = 8 * n + 4 * (lane >> 4);
-            if (t < p.T) of[t] = v[n].x;
-            if (t + 1 < p.T) of[t + 1] = v[n].y;
-            if (t + 2 < p.T) of[t + 2] = v[n].z;
-            if (t + 3 < p.T) of[t + 3] = v[n].w;
+          for (int i = 0; i < kN; ++i) {
+            const int c = 8 * (n0 + i) + col0;
+            if (c < cols) row[c] = v[i].x;
+            if (c + 1 < cols) row[c + 1] = v[i].y;
+            if (c + 2 < cols) row[c + 2] = v[i].z;
+            if (c + 3 < cols) row[c + 3] = v[i].w;
           }
         }
         __syncwarp();
@@ -629,27 +635,21 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       if (kDown) {
         __nv_bfloat16* to = p.out + done.strip * kFewRows + warp * 16 + (lane & 15);
         for (int t = lane >> 4; t < p.T; t += 2) to[static_cast<int64_t>(t) * p.D] = __float2bfloat16_rn(sums[(lane & 15) * pitch + t]);
-      } else if (done.strip * kFewFeatures + r0 < p.F) {
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          if (n >= tiles) break;
-          const float gate[2] = {acc[n][0], acc[n][1]}, up1[2] = {acc[n][2], acc[n][3]};
-          float z[2];
-          swiglu_f32(gate, up1, z, p.act);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int col = 8 * n + 2 * quad + j;
-            if (col < pairs)
-              p.h[static_cast<int64_t>(base + col) * p.F + done.strip * kFewFeatures + r0] = __float2bfloat16_rn(tab.share[base + col] * z[j]);
+      } else {  // eight features of four pairs at a time
+        const int f = done.strip * kFewFeatures + warp * 8 + (lane & 7);
+        const float* row = sums + (lane & 7) * pitch;
+        if (f < p.F)
+#pragma unroll 1
+          for (int col = lane >> 3; col < pairs; col += 4) {
+            const float gate[1] = {row[col]}, up1[1] = {row[8 * pitch + col]};
+            float z[1];
+            swiglu_f32(gate, up1, z, p.act);
+            p.h[static_cast<int64_t>(base + col) * p.F + f] = __float2bfloat16_rn(tab.share[base + col] * z[0]);
           }
-        }
       }
     }
-    if (kDown) {
-      __syncwarp();
-      clear_sums();
-    }
-    clear();
+    __syncwarp();
+    if (kDown) clear_sums();
     whole = true;
     if (work.tickets) {
       const int next = queue.next(ring.abort_flag, lane);
