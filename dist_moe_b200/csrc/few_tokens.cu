@@ -477,8 +477,12 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       x.b[h] = lds16(at_b + here + from[0] + line * 128 + h * 64);
     }
   };
-  auto multiply = [&](float (&to)[4], const Operands& x, const uint4& b, int h) {
+  // 32 values are two instructions.  An instruction waits for the one before it on the same accumulators, and a warp issues in order:
+  // others stand between the two.
+  auto first_half = [&](float (&to)[4], const Operands& x, const uint4& b, int h) {
     mma_16x8x16(to, x.lo[h].x, x.hi[h].x, x.lo[h].y, x.hi[h].y, b.x, b.y);
+  };
+  auto second_half = [&](float (&to)[4], const Operands& x, const uint4& b, int h) {
     mma_16x8x16(to, x.lo[h].z, x.hi[h].z, x.lo[h].w, x.hi[h].w, b.z, b.w);
   };
   auto leave = [&] {  // the item's place is read
@@ -494,7 +498,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
   };
   // `n_items` items in a row with `lines` lines of values.  Beyond them a place holds anything; in the last one zeros follow the values.
   auto run_one_tile = [&](int n_items, int lines) {
-    float odd[4] = {0.f, 0.f, 0.f, 0.f};  // a chain of its own for every second line
+    float more[3][4] = {};
     Operands x, y;
 #pragma unroll 1
     for (int i = 0; i < n_items; ++i, lines -= kFewLines) {
@@ -502,41 +506,60 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       fetch(x, 0);
       if (lines > 1) fetch(y, 1);
       leave();
-      multiply(acc[0], x, x.b[0], 0);
-      multiply(acc[0], x, x.b[1], 1);
+      first_half(acc[0], x, x.b[0], 0);
+      first_half(more[0], x, x.b[1], 1);
       if (lines > 1) {
-        multiply(odd, y, y.b[0], 0);
-        multiply(odd, y, y.b[1], 1);
+        first_half(more[1], y, y.b[0], 0);
+        first_half(more[2], y, y.b[1], 1);
+      }
+      second_half(acc[0], x, x.b[0], 0);
+      second_half(more[0], x, x.b[1], 1);
+      if (lines > 1) {
+        second_half(more[1], y, y.b[0], 0);
+        second_half(more[2], y, y.b[1], 1);
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[0][j] += odd[j];
+    for (int j = 0; j < 4; ++j) acc[0][j] += more[0][j] + (more[1][j] + more[2][j]);
   };
   auto run = [&](int n_items, int lines) {
+    float more[kTiles][4] = {};  // for every second 32 values
     Operands x, y;
-    auto line_of = [&](const Operands& of, int line) {
+    uint4 b[2][4];
+    auto load = [&](uint4 (&to)[4], int n) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 b = of.b[h];
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          if (n >= tiles) break;
-          uint4 next = b;
-          if (n + 1 < kTiles && n + 1 < tiles) next = lds16(at_b + here + from[n + 1 < kTiles ? n + 1 : n] + line * 128 + h * 64);
-          multiply(acc[n], of, b, h);
-          b = next;
-        }
-      }
+      for (int i = 0; i < 4; ++i) to[i] = lds16(at_b + here + from[n] + i * 64);
     };
 #pragma unroll 1
     for (int i = 0; i < n_items; ++i, lines -= kFewLines) {
       wait();
       fetch(x, 0);
-      if (lines > 1) fetch(y, 1);
-      line_of(x, 0);
-      if (lines > 1) line_of(y, 1);
+      fetch(y, 1);
+      if (lines <= 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) y.lo[h] = y.hi[h] = make_uint4(0, 0, 0, 0);
+      }
+      b[0][0] = x.b[0], b[0][1] = x.b[1], b[0][2] = y.b[0], b[0][3] = y.b[1];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        if (n >= tiles) break;
+        const uint4(&now)[4] = b[n & 1];
+        if (n + 1 < kTiles) load(b[(n + 1) & 1], n + 1);
+        first_half(acc[n], x, now[0], 0);
+        first_half(more[n], x, now[1], 1);
+        second_half(acc[n], x, now[0], 0);
+        second_half(more[n], x, now[1], 1);
+        first_half(acc[n], y, now[2], 0);
+        first_half(more[n], y, now[3], 1);
+        second_half(acc[n], y, now[2], 0);
+        second_half(more[n], y, now[3], 1);
+      }
       leave();
     }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[n][j] += more[n][j];
   };
   clear();
   if (kDown) clear_sums();
