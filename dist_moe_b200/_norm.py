@@ -7,7 +7,6 @@ inference call publishes, so that ``routed_experts`` takes them in place of bf16
 from __future__ import annotations
 
 import dataclasses
-import math
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -16,6 +15,7 @@ from . import _native as nat
 from ._call import on_device
 
 _TYPES = (torch.bfloat16, torch.float32)
+_FLOAT32 = torch.finfo(torch.float32)  # what the kernels take eps and the centre as
 
 
 @dataclasses.dataclass(frozen=True, eq=False)
@@ -46,7 +46,7 @@ class QuantizedRows:
         return self.packed[:, self.hidden_dim:self.hidden_dim + self.hidden_dim // 32]
 
     def dequantize(self) -> torch.Tensor:
-        """The rows' values as bf16 ``[T, hidden_dim]`` (exact)."""
+        """The rows' values as bf16 ``[T, hidden_dim]``: exact, but for values below 2 ** -133, which bf16 does not have."""
         T, stride = self.packed.shape
         with on_device(self.packed.device):
             out = torch.empty(T, self.hidden_dim, dtype=torch.bfloat16, device=self.packed.device)
@@ -166,10 +166,10 @@ def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: tor
     device = x_TD.device
     if device.type != "cuda" or weight_D.device != device or (residual_TD is not None and residual_TD.device != device):
         raise ValueError("all operation tensors must reside on the same CUDA device")
-    if not isinstance(eps, (int, float)) or not math.isfinite(eps) or eps <= 0:
-        raise ValueError("eps must be finite and positive")
-    if not isinstance(gain_center, (int, float)) or not math.isfinite(gain_center):
-        raise ValueError("gain_center must be finite")
+    if not isinstance(eps, (int, float)) or not _FLOAT32.tiny <= eps <= _FLOAT32.max:
+        raise ValueError("eps must be finite and positive, in float32 too")
+    if not isinstance(gain_center, (int, float)) or not abs(gain_center) <= _FLOAT32.max:
+        raise ValueError("gain_center must be finite, in float32 too")
     if not isinstance(quantize, bool):
         raise TypeError("quantize must be a bool")
     grads = torch.is_grad_enabled() and (x_TD.requires_grad or weight_D.requires_grad

@@ -2,7 +2,6 @@
 
 from __future__ import annotations
 
-import math
 from typing import Literal
 
 import torch
@@ -93,8 +92,8 @@ def select_experts(logits_TE: torch.Tensor, top_k: int, *, score: Literal["softm
         raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
     if not isinstance(renormalize, bool):
         raise TypeError("renormalize must be a bool")
-    if not isinstance(scale, (int, float)) or not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not isinstance(scale, (int, float)) or not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError("scale must be finite, in float32 too")
     if ids_dtype not in (torch.int32, torch.int64):
         raise TypeError("ids_dtype must be torch.int32 or torch.int64")
     if scores_dtype not in _FLOATS:

@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_gain_kernel(const float* __r
   store1(out + c, sum);
 }
 
-// Packed MXFP8 rows back to bf16, exactly (4 significant bits times a power of two): a warp a row.
+// Packed MXFP8 rows back to bf16, a warp a row: 4 significant bits times a power of two, exact down to bf16's smallest values.
 __global__ void __launch_bounds__(256) mxfp8_dequant_rows_kernel(const uint8_t* __restrict__ rows, int64_t stride, int64_t T, int blocks_of_32,
                                                                  uint4* __restrict__ out) {
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);

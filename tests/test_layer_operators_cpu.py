@@ -30,6 +30,20 @@ def test_add_rms_norm(error, match, args, options):
         dm.add_rms_norm(*args, **options)
 
 
+class _OnDevice(torch.Tensor):
+    """A CPU tensor that says it lies on a GPU: for the checks behind that of the device."""
+
+    device = torch.device("cuda", 0)
+
+
+@pytest.mark.parametrize("options", [dict(eps=v) for v in (0.0, -1e-6, 1e-46, float("inf"), float("nan"), "1")]
+                         + [dict(gain_center=v) for v in (1e39, float("-inf"), float("nan"))])
+def test_add_rms_norm_numbers_that_float32_does_not_hold(options):
+    """An eps that vanishes in float32 would make NaN of a row of zeros."""
+    with pytest.raises(ValueError, match=next(iter(options))):
+        dm.add_rms_norm(_t(2, 8).as_subclass(_OnDevice), _t(8).as_subclass(_OnDevice), **options)
+
+
 @pytest.mark.parametrize("error,match,options", [
     (TypeError, "logits_TE", dict(logits=_t(2, 8, dtype=torch.float16))),
     (ValueError, "logits_TE", dict(logits=_t(8))),
@@ -48,6 +62,8 @@ def test_add_rms_norm(error, match, args, options):
     (ValueError, "score", dict(score="tanh")),
     (TypeError, "renormalize", dict(renormalize=1)),
     (ValueError, "scale", dict(scale=float("inf"))),
+    (ValueError, "scale", dict(scale=float("nan"))),
+    (ValueError, "scale", dict(scale=1e39)),
     (TypeError, "ids_dtype", dict(ids_dtype=torch.int16)),
     (TypeError, "scores_dtype", dict(scores_dtype=torch.float16)),
     (TypeError, "bias_E", dict(bias_E=_t(8))),
