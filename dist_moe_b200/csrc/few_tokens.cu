@@ -605,9 +605,11 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       // What the warps with the same rows do in every block: store their parts, arrive, and the last one finds all parts.
       const int q = kDown ? done.strip : done.a * work.strips + done.strip;  // strip of the product
       const int first = work.split.first_block(q), last = work.split.last_block(q);
-      auto part = [&](int block) {
-        return reinterpret_cast<float4*>(phase.partial) + (work.split.place(block, q) * kFewWarps + warp) * kTiles * 32 + lane;
-      };
+      // The block that a strip begins in keeps it in the second of its places, unless it begins with it; all others in the first.
+      constexpr int kPart = kFewWarps * kTiles * 32;
+      float4* parts = reinterpret_cast<float4*>(phase.partial) + warp * kTiles * 32 + lane;
+      const int first_place = work.split.place(first, q);
+      auto part = [&](int block) { return parts + (block == first ? first_place : 2 * block) * kPart; };
       // A lane's pieces: its row, four columns after another.
       float* row = sums + (lane & 15) * pitch;
       const int col0 = 4 * (lane >> 4), used = (cols + 7) >> 3;
@@ -627,20 +629,26 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
       mine = __shfl_sync(0xffffffffu, before, 0) == last - first;
       if (mine) {
 #pragma unroll 1
-        for (int n0 = 0; n0 < used; n0 += 4) {  // four pieces of several blocks on their way at a time
-          constexpr int kN = kTiles < 4 ? kTiles : 4;
+        for (int n0 = 0; n0 < used; n0 += 4) {
+          // Up to four pieces of four blocks on their way at a time; they are summed in the blocks' order.
+          constexpr int kN = kTiles < 4 ? kTiles : 4, kBlocks = 4;
           float4 v[kN];
 #pragma unroll
           for (int i = 0; i < kN; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll(kN > 2 ? 2 : 4)
-          for (int block = first; block <= last; ++block) {
-            const float4* theirs = part(block) + n0 * 32;
+#pragma unroll 1
+          for (int block = first; block <= last; block += kBlocks) {
+            float4 add[kBlocks][kN];
 #pragma unroll
-            for (int i = 0; i < kN; ++i)
-              if (n0 + i < used) {
-                const float4 add = __ldcg(theirs + i * 32);
-                v[i].x += add.x, v[i].y += add.y, v[i].z += add.z, v[i].w += add.w;
-              }
+            for (int b = 0; b < kBlocks; ++b) {
+              const float4* theirs = part(block + b) + n0 * 32;
+#pragma unroll
+              for (int i = 0; i < kN; ++i)  // beyond `used` a place holds anything
+                add[b][i] = block + b <= last ? __ldcg(theirs + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+              for (int i = 0; i < kN; ++i) v[i].x += add[b][i].x, v[i].y += add[b][i].y, v[i].z += add[b][i].z, v[i].w += add[b][i].w;
           }
 #pragma unroll
           for (int i = 0; i < kN; ++i) {
@@ -656,8 +664,12 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
     }
     if (mine) {
       if (kDown) {
-        __nv_bfloat16* to = p.out + done.strip * kFewRows + warp * 16 + (lane & 15);
-        for (int t = lane >> 4; t < p.T; t += 2) to[static_cast<int64_t>(t) * p.D] = __float2bfloat16_rn(sums[(lane & 15) * pitch + t]);
+        // two columns of four tokens at a time
+        const float* row = sums + 2 * (lane & 7) * pitch;
+        __nv_bfloat16* to = p.out + done.strip * kFewRows + warp * 16 + 2 * (lane & 7);
+#pragma unroll 2
+        for (int t = lane >> 3; t < p.T; t += 4)
+          *reinterpret_cast<uint32_t*>(to + static_cast<int64_t>(t) * p.D) = pack_bf16x2(row[t], row[pitch + t]);
       } else {  // eight features of four pairs at a time
         const int f = done.strip * kFewFeatures + warp * 8 + (lane & 7);
         const float* row = sums + (lane & 7) * pitch;
@@ -825,7 +837,7 @@ extern "C" int dm_few_tokens(const void* x, const void* ids, int ids_are_int64, 
   if (!x || !ids || !scores || !w13 || !w2 || !out || !workspace) return kRcBadArg;
   int rc = few_shape(T, D, F, E, K);
   if (rc != kRcOk) return rc;
-  for (const void* v : {x, w13, w2, static_cast<const void*>(workspace)})
+  for (const void* v : {x, w13, w2, static_cast<const void*>(out), static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(v) % 16 != 0) return kRcBadArg;
   const FewLayout l = few_layout(T, F, K);
   if (workspace_bytes < l.total) return kRcBadArg;

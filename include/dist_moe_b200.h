@@ -717,10 +717,10 @@ int dm_select_experts_bwd(const void* logits, int logits_are_bf16, int64_t strid
 
 /* dm_few_tokens: the whole layer for up to DM_FEW_TOKENS_MAX tokens with bf16 weights, all experts local, in one cooperative launch.
  * out[t] = sum_e c[t, e] W2[e] SwiGLU(W13[e] x[t]), c[t, e] = sum of the scores of token t's routes to expert e.  ids outside
- * [0, E) go nowhere, other than -1 they are reported in `status`.  D % 64 == 0, F % 8 == 0, E <= 1024, K <= 32.  The workspace
- * (dm_few_tokens_workspace_bytes, on the device of the launch; a negative DM_RC_* for an unsupported shape) belongs to one call at a
- * time; its first DM_FEW_TOKENS_COUNTER_BYTES are zeroed once before its first use, and after a call that reported
- * DM_STATUS_PIPELINE_TIMEOUT. */
+ * [0, E) go nowhere, other than -1 they are reported in `status`.  D % 64 == 0, F % 8 == 0, E <= 1024, K <= 32; x, weights, out and
+ * workspace are 16-byte aligned.  The workspace (dm_few_tokens_workspace_bytes, on the device of the launch; a negative DM_RC_* for an
+ * unsupported shape) belongs to one call at a time; its first DM_FEW_TOKENS_COUNTER_BYTES are zeroed once before its first use, and
+ * after a call that reported DM_STATUS_PIPELINE_TIMEOUT. */
 #define DM_FEW_TOKENS_MAX 64
 #define DM_FEW_TOKENS_COUNTER_BYTES 8192
 int64_t dm_few_tokens_workspace_bytes(int64_t T, int64_t D, int64_t F, int E, int K);

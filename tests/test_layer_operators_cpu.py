@@ -141,6 +141,6 @@ def test_entry_points_return_codes():
     size = lib.dm_few_tokens_workspace_bytes
     assert size(65, 64, 32, 4, 2) == -3 and size(1, 64, 32, 1025, 2) == -3 and size(1, 64, 32, 64, 33) == -3
     assert size(1, 64, 12, 4, 2) == -2 and size(1, 48, 16, 4, 2) == -2 and size(0, 64, 32, 4, 2) == -1 and size(64, 64, 32, 4, 2) > 0
-    few = lambda x=some, ws=some, n=1 << 40, T=1: lib.dm_few_tokens(  # noqa: E731
-        x, some, 0, some, 0, some, some, some, T, 64, 32, 4, 2, 0, 1.0, 0.0, ws, n, 0, None, None)
-    assert few(x=None) == -1 and few(x=some + 8) == -1 and few(n=16) == -1 and few(T=65) == -3 and few(ws=None) == -1
+    few = lambda x=some, ws=some, n=1 << 40, T=1, out=some: lib.dm_few_tokens(  # noqa: E731
+        x, some, 0, some, 0, some, some, out, T, 64, 32, 4, 2, 0, 1.0, 0.0, ws, n, 0, None, None)
+    assert few(x=None) == -1 and few(x=some + 8) == -1 and few(out=some + 2) == -1 and few(n=16) == -1 and few(T=65) == -3 and few(ws=None) == -1
