@@ -215,6 +215,46 @@ def test_captured_calls_replay_on_new_tokens_between_eager_ones():
     ctx.close()
 
 
+def test_experts_that_lie_behind_32_bit_offsets():
+    T, D, F, E, K, last = 6, 2048, 1408, 500, 3, 5
+    case = _case(T, D, F, last, K)
+    w13, w2 = (torch.empty(E, *t.shape[1:], device=DEV, dtype=t.dtype) for t in case[3:])
+    w13[-last:], w2[-last:] = case[3], case[4]
+    assert w13.numel() > 2 ** 31 and w2.numel() * 2 > 2 ** 31
+    ctx, small = _context(T, D, F, E, K), _context(T, D, F, last, K)
+    want = dm.routed_experts_few_tokens(*case, small)
+    _check(want, case)
+    assert torch.equal(dm.routed_experts_few_tokens(case[0], case[1] + (E - last), case[2], w13, w2, ctx), want)
+    for c in (ctx, small):
+        c.check_status()
+        c.close()
+
+
+@pytest.mark.parametrize("priority", [0, -1])
+def test_contexts_at_the_same_time(priority):
+    """Two contexts on two streams, beside products that hold SMs: every launch gets all of its blocks."""
+    T, D, F, E, K = 12, 512, 1408, 16, 4
+    cases = [_case(T, D, F, E, K, seed=i) for i in range(2)]
+    contexts = [_context(T, D, F, E, K) for _ in cases]
+    want = [dm.routed_experts_few_tokens(*case, ctx) for case, ctx in zip(cases, contexts)]
+    a = torch.randn(2048, 2048, device=DEV).bfloat16()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream(priority=priority), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(50):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(dm.routed_experts_few_tokens(*cases[i], contexts[i]))
+        with torch.cuda.stream(streams[2]):
+            b = a @ a
+    torch.cuda.synchronize()
+    for i, ctx in enumerate(contexts):
+        ctx.check_status()
+        assert all(torch.equal(g, want[i]) for g in got[i])
+        ctx.close()
+    del b
+
+
 def test_refusals_that_need_a_device():
     T, D, F, E, K = 4, 128, 64, 4, 2
     x, ids, scores, w13, w2 = _case(T, D, F, E, K)
