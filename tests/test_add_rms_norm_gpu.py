@@ -237,3 +237,30 @@ def test_same_bits_every_time_and_on_another_stream():
         again = torch.autograd.grad(dm.add_rms_norm(x, w, residual_TD=r)[0], w, gy)[0]
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(first, again)
+
+
+def test_rows_behind_32_bit_offsets():
+    D, last = 8192, 5
+    T = 2 ** 31 // D + 100
+    w = torch.rand(D, device=DEV)
+    x, gy = (torch.zeros(T, D, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    for t in (x, gy):
+        t[-last:] = torch.randn(last, D, device=DEV)
+    few = [t[-last:].clone().requires_grad_() for t in (x, x)] + [w.clone().requires_grad_()]
+    many = [x.requires_grad_(), x.detach().clone().requires_grad_(), w.requires_grad_()]
+    got = []
+    for a, r, g in (many, few):
+        y, total = dm.add_rms_norm(a, g, residual_TD=r)
+        ga, gr, gg = torch.autograd.grad((y, total), (a, r, g), (gy[-len(a):], gy[-len(a):]))
+        got.append([t[-last:].clone() for t in (y, total, ga, gr)] + [gg])
+        del y, total, ga, gr
+    for a, b in zip(got[0][:4], got[1][:4]):
+        assert torch.equal(a, b)
+    # The other rows add zeros.  The five meet in another order: two roundings of a product and four of sums on either side, 2^-24 each
+    # of the sum of |gy s rstd|, and |s rstd| is at most sqrt(D).
+    bound = 12 * 2.0 ** -24 * D ** 0.5 * gy[-last:].double().abs().sum(0)
+    assert bool(((got[0][4].double() - got[1][4].double()).abs() <= bound).all())
+    with torch.no_grad():
+        rows = dm.add_rms_norm(x, w, residual_TD=x, quantize=True)[2]
+        want = dm.add_rms_norm(x[-last:].clone(), w, residual_TD=x[-last:].clone(), quantize=True)[2]
+        assert torch.equal(rows.packed[-last:], want.packed)

@@ -238,3 +238,19 @@ def test_layouts_streams_capture_and_no_tokens():
     graph.replay()
     want = dm.select_experts(logits, 8)
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_rows_behind_32_bit_offsets():
+    E, K, last = 1024, 8, 7
+    T = 2 ** 31 // E + 100
+    logits = torch.zeros(T, E, device=DEV, dtype=torch.bfloat16)
+    logits[-last:] = torch.randn(last, E, device=DEV)
+    few = logits[-last:].clone()
+    got = []
+    for l in (logits, few):
+        l.requires_grad_()
+        ids, scores = dm.select_experts(l, K)
+        grad, = torch.autograd.grad(scores, l, torch.ones_like(scores))
+        got.append([t[-last:].clone() for t in (ids, scores, grad)])
+        del ids, scores, grad
+    assert all(torch.equal(a, b) for a, b in zip(*got))
