@@ -9,9 +9,11 @@
 //
 // HBM bound: every value of a row stays in registers between its sum and its use, 2 + 2|4 bytes in and 2 + 2|4 (+ 1.03) out per
 // element, in the backward 2 + 2|4 + 2|4 in and 2 (+ 4) out.  A row of up to 1024 values belongs to a warp, four 16-byte pieces a lane,
-// four rows to a block; a longer one to a block of as many warps as it takes with two pieces a lane (four beyond 8192 values): with
-// 128, 256 or 512 threads for lengths in between, a third of the lanes idle, 4096 rows of 2816 took the backward 30 and 55 us.  The gain's gradient is summed
-// over the rows of a block in registers and over the blocks by a second launch, always in the same order.
+// four rows to a block; a longer one to a block of as many warps as it takes with two pieces a lane (four beyond 8192 values).  The
+// gain's gradient is summed over the rows of a block in registers and over the blocks by a second launch, always in the same order.
+//
+// Measured, L2 flushed, events included (some 6 us): 16384 x 4096 bf16 forward 96 us (5.6 TB/s), backward 116 us with the gain's gradient,
+// 107 without; 4096 x 2816 with an fp32 stream 29 us, with quantised rows 31 us, backward 58 us; 16 x 2048 8 us.
 #include <type_traits>
 
 #include "quant_common.cuh"
@@ -176,7 +178,8 @@ __global__ void __launch_bounds__(256) add_rmsnorm_fwd_any_kernel(
 }
 
 // A backward block keeps kStages rows (of four warps each its own) on their way in shared memory, as 16-byte pieces that the thread
-// which asked for them reads back itself: no barrier stands between a copy and its use.
+// which asked for them reads back itself: no barrier stands between a copy and its use.  A row's arithmetic needs its sum first, so
+// without the next rows on their way the loads stop for it.
 template <typename R, int kVec>
 struct NormBwd {
   static constexpr int kWide = sizeof(R) / 2;  // 16-byte pieces of eight values of the stream

@@ -8,15 +8,20 @@
 // HBM bound: the weights of every expert that is hit stream through once (6 D F bytes each), all else is small.  So the weights never
 // wait: one warp of a block brings them into a ring in shared memory (an item by one tensor copy) and goes on from W13 to W2 at once,
 // another brings the rows of x or h that meet them (512 bytes by one cp.async of the warp) and alone waits for the other blocks where
-// h begins: by then 200 KB of W2 per SM are there.  All blocks are resident at once (cooperative launch), and that wait is bounded.
+// h begins: by then up to 200 KB of W2 per SM are there.  All blocks are resident at once (cooperative launch), and that wait is bounded.
+//
+// Measured as replayed graphs, L2 flushed, beside what the weights take at the copy rate: 64 experts x 2048 x 1408, top 6, 1 token 39 us
+// (16), 4 tokens 86 (55), 32 tokens 180 (158), 64 tokens 220 (169); 32 experts x 7168 x 2048, top 8, 4 tokens 301 to 307 (295).  With
+// sixteen tokens to an expert the products hold it, not the stream: 64 tokens of that layer 700 (430).  Of a call with little to read,
+// 3 us go by before the first product, 2 us at the meeting, and 4 to 5 us on the parts of cut strips at the end.
 //
 // A block works on strips of 64 weight rows (32 features of gate and up; 64 output columns), 16 for each of its four warps that multiply;
 // an item is 128 values of the inner dimension of a strip, 16 KiB.  A warp has its rows for itself, sums them in registers and ends a
 // strip without the others: nothing but the ring's places keeps the warps together.  (With the inner dimension of an item shared by
-// eight warps, the barrier and the sums in shared memory at the end of a strip stopped the stream: 32 tokens of 64 experts x 2048 x 1408
-// took 207 us, 176 without them.)  Where W13 has enough strips, blocks take them by tickets; else, and for W2, the items of all strips
-// are dealt out evenly over the blocks, whatever the number of experts hit.  Rows of a strip that is cut between blocks are summed by
-// the one of the blocks' warps that finishes last, in the order of the blocks.
+// eight warps, the barrier and the sums in shared memory at the end of a strip stopped the stream: the 32 tokens above took 207 us.)
+// Where W13 has enough strips, blocks take them by tickets; else, and for W2, the items of all strips are dealt out evenly over the
+// blocks, whatever the number of experts hit.  Rows of a strip that is cut between blocks are summed by the one of the blocks' warps
+// that finishes last, in the order of the blocks.
 //
 // With so few columns the products are mma.sync m16n8k16, weights as the 16-row operand, tokens as the 8 columns: both operands are
 // then read 16 bytes a lane along the inner dimension as they lie in shared memory, its order inside 32 values being the same for both
@@ -257,10 +262,13 @@ struct FewCursor {
   }
 };
 
-// Whole strips by tickets, where the last round of them is full enough.
+// Whole strips by tickets, where the rounds are three quarters full or more on average: nothing is cut then, and blocks that are served
+// faster take more.  Even shares took 2 to 5 % longer from 0.74 full up in 2 to 5 rounds, 10 % in 10 and more (32 tokens of 64 experts x
+// 2048 x 1408 199 us against 181, 4 of 32 x 7168 x 2048 336 against 307); tickets took 3 % longer at 0.72 and 9 % at 0.65 (5 and 3
+// experts x 7168 x 2048).
 __device__ __forceinline__ bool few_by_tickets(uint32_t strips, uint32_t blocks) {
   const uint64_t rounds = (strips + blocks - 1) / blocks;
-  return 5ull * strips >= 4 * rounds * blocks;
+  return 4ull * strips >= 3 * rounds * blocks;
 }
 
 // What the warps of a block know of one of the two products.
@@ -421,10 +429,10 @@ __device__ __noinline__ void few_wait_on(uint64_t* bar, uint32_t parity, int* ab
 }
 
 // The warps that multiply.  kTiles: tiles of eight columns that the accumulators hold.  Columns are an expert's tokens, next to one
-// another.  At the end of a strip the sums go through shared memory (the code for every tile's activation or partial sums in a row made
-// the launch slower: what the warps run has to stay small); W2, which sums over the experts, adds them there by token after each expert.  (With all tokens
-// as W2's columns, zero where they are not the expert's, 32 and 64 tokens of the layer above took 230 and 370 us where 215 and 285 were
-// reached, and a weight that is not finite reached every token.)
+// another.  At the end of a strip the sums go through shared memory; W2, which sums over the experts, adds them there by token after each
+// expert.  (With all tokens as W2's columns, zero where they are not the expert's, 32 and 64 tokens of the layer above took 15 and 85 us
+// more, and a weight that is not finite reached every token.)  What the warps run has to stay small: most of it runs a few times only,
+// from instruction memory, and every tile's activation or partial sums written out in a row made the launch slower.
 template <bool kDown, int kTiles>
 __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables& tab, FewRing& ring, FewQueue& queue, int active, float* all_sums) {
   FewWork<kDown> work(p, active);

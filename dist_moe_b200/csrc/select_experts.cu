@@ -19,6 +19,9 @@
 //
 // A warp per token: its logits sit in registers, expert 32 j + lane in register j.  Each of the K rounds is two warp reductions over the
 // lanes' largest remaining values; a lane keeps its two largest, and looks through its registers again where a third is asked for.
+//
+// Instruction bound: the logits are read once (4096 x 256 in 0.6 us at the copy rate).  Measured, events included (some 6 us), K = 8:
+// 4096 x 256 12 us from the logits alone, 14 with a bias, 17 with 4 of 8 groups too, 16384 x 256 27 and 47; backward 8 to 10 and 18.
 #include <type_traits>
 
 #include "common.cuh"
@@ -81,9 +84,6 @@ __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
   }
   return k;
 }
-
-__device__ __forceinline__ float exp_v(float x) { return expf(x); }
-__device__ __forceinline__ double exp_v(double x) { return exp(x); }
 
 // What the softmax's exponential is taken of: +inf logits, which are the largest then, share it.
 template <typename V>
