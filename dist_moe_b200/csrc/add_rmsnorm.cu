@@ -8,9 +8,11 @@
 // D bytes E4M3, D / 32 scale bytes, padding to 16 bytes.
 //
 // HBM bound: every value of a row stays in registers between its sum and its use, 2 + 2|4 bytes in and 2 + 2|4 (+ 1.03) out per
-// element, in the backward 2 + 2|4 + 2|4 in and 2 (+ 4) out.  A row of up to 1024 values belongs to a warp, four 16-byte pieces a lane,
-// four rows to a block; a longer one to a block of as many warps as it takes with two pieces a lane (four beyond 8192 values).  The
-// gain's gradient is summed over the rows of a block in registers and over the blocks by a second launch, always in the same order.
+// element, in the backward 2 + 2|4 + 2|4 in and 2 (+ 4) out.  A row belongs to a block of as many warps as it takes with two 16-byte
+// pieces a lane (four beyond 8192 values); in the backward one of up to 1024 values to a warp, four pieces a lane, four rows to a block:
+// 16384 rows of 256 and 1024 values took 28 and 47 us so, 36 and 50 with blocks (in the forward 15 and 32 with warps, 15 and 30 with
+// blocks).  The gain's gradient is summed over the rows of a block in registers and over the blocks by a second launch, always in the
+// same order.
 //
 // Measured, L2 flushed, events included (some 6 us): 16384 x 4096 bf16 forward 96 us (5.6 TB/s), backward 116 us with the gain's gradient,
 // 107 without; 4096 x 2816 with an fp32 stream 29 us, with quantised rows 31 us, backward 58 us; 16 x 2048 8 us.
@@ -98,14 +100,13 @@ __device__ __forceinline__ void quantise_piece(const uint4& y, int v, bool in, i
 }
 
 // kVec pieces of 8 values a thread.
-template <typename R, bool kResidual, bool kWarpRow, int kVec>
-__global__ void __launch_bounds__(kWarpRow ? 128 : kNormThreads) add_rmsnorm_fwd_kernel(
+template <typename R, bool kResidual, int kVec>
+__global__ void __launch_bounds__(kNormThreads) add_rmsnorm_fwd_kernel(
     const __nv_bfloat16* __restrict__ x, int64_t x_stride, const R* __restrict__ residual, int64_t r_stride, Gain gain, float eps,
-    int64_t T, int vec, R* __restrict__ sum_out, __nv_bfloat16* __restrict__ y_out, float* __restrict__ rstd_out, QuantRows quant) {
+    int vec, R* __restrict__ sum_out, __nv_bfloat16* __restrict__ y_out, float* __restrict__ rstd_out, QuantRows quant) {
   __shared__ float part[kNormThreads / 32];
-  const int threads = kWarpRow ? 32 : blockDim.x, lane = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t t = kWarpRow ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  if (t >= T) return;  // whole warps
+  const int threads = blockDim.x, lane = threadIdx.x;
+  const int64_t t = blockIdx.x;
   const int64_t D = static_cast<int64_t>(vec) * 8;
   float s[kVec][8];
   float ss = 0.f;
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : kNormThreads) add_rmsnorm_fwd
   for (int i = 0; i < kVec; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss += s[i][j] * s[i][j];
-  const float rstd = rsqrtf(row_sum<kWarpRow>(ss, part) / static_cast<float>(D) + eps);
+  const float rstd = rsqrtf(row_sum<false>(ss, part) / static_cast<float>(D) + eps);
   if (rstd_out != nullptr && lane == 0) rstd_out[t] = rstd;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
@@ -420,13 +421,12 @@ static int add_rmsnorm_fwd(const void* x, int64_t x_stride, const void* residual
     return static_cast<int>(cudaGetLastError());
   }
   const int vec = static_cast<int>(D / 8);
-  auto run = [&](auto kernel, unsigned blocks, int threads) {
-    kernel<<<blocks, threads, 0, st>>>(xp, x_stride, rp, r_stride, gain, eps, T, vec, sp, yp, rstd_out, quant);
+  auto run = [&](auto kernel, int threads) {
+    kernel<<<static_cast<unsigned>(T), threads, 0, st>>>(xp, x_stride, rp, r_stride, gain, eps, vec, sp, yp, rstd_out, quant);
     return static_cast<int>(cudaGetLastError());
   };
-  if (D <= 1024) return run(add_rmsnorm_fwd_kernel<R, kResidual, true, 4>, static_cast<unsigned>(ceil_div64(T, 4)), 128);
-  if (vec <= 2 * kNormThreads) return run(add_rmsnorm_fwd_kernel<R, kResidual, false, 2>, static_cast<unsigned>(T), norm_threads(vec, 2));
-  return run(add_rmsnorm_fwd_kernel<R, kResidual, false, 4>, static_cast<unsigned>(T), norm_threads(vec, 4));
+  if (vec <= 2 * kNormThreads) return run(add_rmsnorm_fwd_kernel<R, kResidual, 2>, norm_threads(vec, 2));
+  return run(add_rmsnorm_fwd_kernel<R, kResidual, 4>, norm_threads(vec, 4));
 }
 
 extern "C" int dm_add_rmsnorm_fwd(const void* x, int64_t x_stride, const void* residual, int residual_is_f32, int64_t residual_stride,
@@ -480,10 +480,9 @@ static int add_rmsnorm_bwd(const void* grad_y, const void* grad_sum, const void*
     return static_cast<int>(cudaGetLastError());
   };
   using std::integral_constant;
-  // Three stages where four blocks of them fit on an SM, else two, else one (rows of more than 8192 values with an fp32 stream).
+  // Two stages (three were not faster), or one where they do not fit: rows of more than 8192 values with an fp32 stream.
   auto run = [&](auto warp_tag, auto vec_tag, int threads) {
     using C = NormBwd<R, decltype(vec_tag)::value>;
-    if (C::resident(threads, 3) == 4) return launch(warp_tag, vec_tag, integral_constant<int, 3>{}, threads);
     if (C::resident(threads, 2) >= 1) return launch(warp_tag, vec_tag, integral_constant<int, 2>{}, threads);
     return launch(warp_tag, vec_tag, integral_constant<int, 1>{}, threads);
   };
