@@ -161,8 +161,9 @@ class ContextState:
         same time (calls on one context have to be ordered) may have left some of them behind, and later ones would take rows for
         gathered that are not."""
         self.gather_flags.zero_()
-        if self.few_workspace is not None:
-            self.few_workspace[:_few_tokens.COUNTER_BYTES].zero_()
+        few = getattr(self, "few_workspace", None)
+        if few is not None:
+            few[:_few_tokens.COUNTER_BYTES].zero_()
 
     def select_slot(self, slot: int, num_layers: int) -> None:
         if self.num_slots == 0:
