@@ -13,7 +13,7 @@
 // Measured as replayed graphs, L2 flushed, beside what the weights take at the copy rate: 64 experts x 2048 x 1408, top 6, 1 token 39 us
 // (16), 4 tokens 86 (55), 32 tokens 180 (158), 64 tokens 220 (169); 32 experts x 7168 x 2048, top 8, 4 tokens 301 to 307 (295).  With
 // sixteen tokens to an expert the products hold it, not the stream: 64 tokens of that layer 700 (430).  Of a call with little to read,
-// 3 us go by before the first product, 2 us at the meeting, and 4 to 5 us on the parts of cut strips at the end.
+// 3 us go by before the first product, 1 to 2 at the meeting, and 2 to 5 on the parts of cut strips at the end.
 //
 // A block works on strips of 64 weight rows (32 features of gate and up; 64 output columns), 16 for each of its four warps that multiply;
 // an item is 128 values of the inner dimension of a strip, 16 KiB.  A warp has its rows for itself, sums them in registers and ends a
