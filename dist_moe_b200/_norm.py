@@ -105,8 +105,13 @@ class _AddRmsNorm(torch.autograd.Function):
         return y if residual is None else (y, total)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y, grad_sum=None):
+        if torch.is_grad_enabled():  # create_graph=True: differentiating the gradients raises
+            return _AddRmsNorm._backward_once(ctx, grad_y, grad_sum)
+        return _AddRmsNorm._backward(ctx, grad_y, grad_sum)
+
+    @staticmethod
+    def _backward(ctx, grad_y, grad_sum):
         want_x, want_residual, want_weight = ctx.needs_input_grad[:3]
         total, weight, rstd = ctx.saved_tensors
         if grad_y is None:  # the stream alone is differentiated
@@ -122,11 +127,11 @@ class _AddRmsNorm(torch.autograd.Function):
             if grad_sum is not None:
                 grad_sum = grad_sum.contiguous()
             gx = torch.empty_like(grad_y) if want_x or (want_residual and not apart) else None
-            gr = torch.empty((T, D), dtype=torch.float32, device=device) if want_residual and apart else None
+            gr = torch.empty_like(total) if want_residual and apart else None
             gw = partial = None
             if want_weight:
                 gw = torch.empty_like(weight)
-                partial = torch.empty((nat.lib.dm_add_rmsnorm_shares(T, D), D), dtype=torch.float32, device=device)
+                partial = rstd.new_empty((nat.lib.dm_add_rmsnorm_shares(T, D), D))
             if T == 0:
                 gw = gw.zero_() if want_weight else None
             else:
@@ -135,6 +140,8 @@ class _AddRmsNorm(torch.autograd.Function):
                     weight.dtype is torch.float32, ctx.center, rstd.data_ptr(), T, D, nat.ptr(gx), nat.ptr(gr), nat.ptr(partial),
                     nat.ptr(gw), nat.stream_ptr()), "dm_add_rmsnorm_bwd", 2 if want_weight else 1)
         return gx if want_x else None, (gr if apart else gx) if want_residual else None, gw, None, None
+
+    _backward_once = staticmethod(once_differentiable(_backward.__func__))
 
 
 def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: torch.Tensor | None = None, eps: float = 1e-6,

@@ -38,8 +38,13 @@ class _SelectExperts(torch.autograd.Function):
         return ids, scores
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, _, grad_scores):
+    def backward(ctx, grad_ids, grad_scores):
+        if torch.is_grad_enabled():  # create_graph=True: differentiating the gradients raises
+            return _SelectExperts._backward_once(ctx, grad_ids, grad_scores)
+        return _SelectExperts._backward(ctx, grad_ids, grad_scores)
+
+    @staticmethod
+    def _backward(ctx, _, grad_scores):
         if grad_scores is None:
             return None, None
         logits, ids = ctx.saved_tensors
@@ -47,12 +52,14 @@ class _SelectExperts(torch.autograd.Function):
         T, E = logits.shape
         with on_device(logits.device):
             grad_scores = grad_scores.contiguous()
-            out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+            out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((T, E), dtype=logits.dtype, device=logits.device)
             nat.check(nat.lib.dm_select_experts_bwd(
                 logits.data_ptr(), logits.dtype is torch.bfloat16, logits.stride(0), T, E, top_k, sigmoid, renormalize, scale,
                 ids.data_ptr(), ids.dtype is torch.int64, grad_scores.data_ptr(), grad_scores.dtype is torch.bfloat16,
                 out.data_ptr(), nat.stream_ptr()), "dm_select_experts_bwd", int(T > 0))
         return out, None
+
+    _backward_once = staticmethod(once_differentiable(_backward.__func__))
 
 
 def select_experts(logits_TE: torch.Tensor, top_k: int, *, score: Literal["softmax", "sigmoid"] = "softmax",

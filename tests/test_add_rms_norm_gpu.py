@@ -264,3 +264,14 @@ def test_rows_behind_32_bit_offsets():
         rows = dm.add_rms_norm(x, w, residual_TD=x, quantize=True)[2]
         want = dm.add_rms_norm(x[-last:].clone(), w, residual_TD=x[-last:].clone(), quantize=True)[2]
         assert torch.equal(rows.packed[-last:], want.packed)
+
+
+def test_gradients_are_not_differentiated_again():
+    x, r, w = (t.requires_grad_() for t in _inputs(5, 256, torch.float32, torch.float32, 0.0))
+    y, total = dm.add_rms_norm(x, w, residual_TD=r)
+    loss = y.float().pow(2).sum() + total.sum()
+    first = torch.autograd.grad(loss, (x, r, w), retain_graph=True)
+    again = torch.autograd.grad(loss, (x, r, w), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, again)) and again[0].requires_grad
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        again[1].sum().backward()

@@ -254,3 +254,13 @@ def test_rows_behind_32_bit_offsets():
         got.append([t[-last:].clone() for t in (ids, scores, grad)])
         del ids, scores, grad
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_gradients_are_not_differentiated_again():
+    logits = torch.randn(5, 16, device=DEV, requires_grad=True)
+    loss = dm.select_experts(logits, 4)[1].pow(2).sum()
+    first, = torch.autograd.grad(loss, logits, retain_graph=True)
+    again, = torch.autograd.grad(loss, logits, create_graph=True)
+    assert torch.equal(first, again) and again.requires_grad
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        again.sum().backward()
