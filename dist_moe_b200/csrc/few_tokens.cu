@@ -635,6 +635,7 @@ __device__ __forceinline__ void few_multiply(const FewParams& p, const FewTables
         if (before == last - first) *arrived = 0;  // clear for the next call
       }
       mine = __shfl_sync(0xffffffffu, before, 0) == last - first;
+      __syncwarp();  // what lane 0 acquired the other lanes read: a shuffle does not order memory
       if (mine) {
 #pragma unroll 1
         for (int n0 = 0; n0 < used; n0 += 4) {
