@@ -91,6 +91,24 @@ def on_device(device: torch.device):
     return _NOTHING if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, name, grads, *sources):
+        ctx.operation = name
+        return tuple(None if g is None else g.clone() for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"trying to differentiate twice {ctx.operation}, whose gradients have no derivative")
+
+
+def differentiable_once(name: str, grads: tuple, sources: tuple) -> tuple:
+    """The gradients of a backward pass that is recorded itself (``create_graph=True``), tied to what they were computed from by a node
+    that raises.  ``once_differentiable`` ties them to nothing: where the incoming gradients are constants, or where the second
+    derivative is asked for by its leaves, it leaves a term out without a word."""
+    return _Once.apply(name, grads, *sources)
+
+
 def launch(fn, names: dict, state, k, steps: int) -> None:
     """Run the given steps of a sequence: one call, or one per step where they are timed in place."""
     context, st = state.native_layer(), nat.stream_ptr()

@@ -9,10 +9,9 @@ from __future__ import annotations
 import dataclasses
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from ._call import on_device
+from ._call import differentiable_once, on_device
 
 _TYPES = (torch.bfloat16, torch.float32)
 _FLOAT32 = torch.finfo(torch.float32)  # what the kernels take eps and the centre as
@@ -106,12 +105,6 @@ class _AddRmsNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y, grad_sum=None):
-        if torch.is_grad_enabled():  # create_graph=True: differentiating the gradients raises
-            return _AddRmsNorm._backward_once(ctx, grad_y, grad_sum)
-        return _AddRmsNorm._backward(ctx, grad_y, grad_sum)
-
-    @staticmethod
-    def _backward(ctx, grad_y, grad_sum):
         want_x, want_residual, want_weight = ctx.needs_input_grad[:3]
         total, weight, rstd = ctx.saved_tensors
         if grad_y is None:  # the stream alone is differentiated
@@ -119,29 +112,38 @@ class _AddRmsNorm(torch.autograd.Function):
                 return None, None, None, None, None
             return (grad_sum.to(torch.bfloat16) if want_x else None, grad_sum if want_residual else None,
                     torch.zeros_like(weight) if want_weight else None, None, None)
-        T, D = grad_y.shape
-        device = grad_y.device
-        apart = total.dtype is torch.float32
-        with on_device(device):
-            grad_y = grad_y.contiguous()
-            if grad_sum is not None:
-                grad_sum = grad_sum.contiguous()
-            gx = torch.empty_like(grad_y) if want_x or (want_residual and not apart) else None
-            gr = torch.empty_like(total) if want_residual and apart else None
-            gw = partial = None
-            if want_weight:
-                gw = torch.empty_like(weight)
-                partial = rstd.new_empty((nat.lib.dm_add_rmsnorm_shares(T, D), D))
-            if T == 0:
-                gw = gw.zero_() if want_weight else None
-            else:
-                nat.check(nat.lib.dm_add_rmsnorm_bwd(
-                    grad_y.data_ptr(), nat.ptr(grad_sum), total.data_ptr(), apart, total.stride(0), weight.data_ptr(),
-                    weight.dtype is torch.float32, ctx.center, rstd.data_ptr(), T, D, nat.ptr(gx), nat.ptr(gr), nat.ptr(partial),
-                    nat.ptr(gw), nat.stream_ptr()), "dm_add_rmsnorm_bwd", 2 if want_weight else 1)
-        return gx if want_x else None, (gr if apart else gx) if want_residual else None, gw, None, None
+        if not torch.is_grad_enabled():
+            return *_backward(ctx, grad_y, grad_sum, total, weight, rstd), None, None
+        with torch.no_grad():
+            gx, gr, gw = _backward(ctx, grad_y, grad_sum, total, weight, rstd)
+        gx, gr = differentiable_once("add_rms_norm", (gx, gr), (grad_y, grad_sum, total, weight))
+        gw, = differentiable_once("add_rms_norm", (gw,), (grad_y, total if want_x or want_residual else None))
+        return gx, gr, gw, None, None
 
-    _backward_once = staticmethod(once_differentiable(_backward.__func__))
+
+def _backward(ctx, grad_y, grad_sum, total, weight, rstd):
+    want_x, want_residual, want_weight = ctx.needs_input_grad[:3]
+    T, D = grad_y.shape
+    device = grad_y.device
+    apart = total.dtype is torch.float32
+    with on_device(device):
+        grad_y = grad_y.contiguous()
+        if grad_sum is not None:
+            grad_sum = grad_sum.contiguous()
+        gx = torch.empty_like(grad_y) if want_x or (want_residual and not apart) else None
+        gr = torch.empty_like(total) if want_residual and apart else None
+        gw = partial = None
+        if want_weight:
+            gw = torch.empty_like(weight)
+            partial = rstd.new_empty((nat.lib.dm_add_rmsnorm_shares(T, D), D))
+        if T == 0:
+            gw = gw.zero_() if want_weight else None
+        else:
+            nat.check(nat.lib.dm_add_rmsnorm_bwd(
+                grad_y.data_ptr(), nat.ptr(grad_sum), total.data_ptr(), apart, total.stride(0), weight.data_ptr(),
+                weight.dtype is torch.float32, ctx.center, rstd.data_ptr(), T, D, nat.ptr(gx), nat.ptr(gr), nat.ptr(partial),
+                nat.ptr(gw), nat.stream_ptr()), "dm_add_rmsnorm_bwd", 2 if want_weight else 1)
+    return gx if want_x else None, (gr if apart else gx) if want_residual else None, gw
 
 
 def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: torch.Tensor | None = None, eps: float = 1e-6,
@@ -189,8 +191,10 @@ def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: tor
     if not weight_D.is_contiguous():
         weight_D = weight_D.contiguous()
     if grads:
-        got = _AddRmsNorm.apply(x_TD, residual_TD, weight_D, float(eps), float(gain_center))
-        return got if residual_TD is not None else (got, x_TD)
+        if residual_TD is None:
+            kept = _rows(x_TD)  # what is saved is what the gradients depend on
+            return _AddRmsNorm.apply(kept, None, weight_D, float(eps), float(gain_center)), x_TD
+        return _AddRmsNorm.apply(x_TD, residual_TD, weight_D, float(eps), float(gain_center))
     with on_device(device):
         if quantize:  # the quantiser's 16-byte pieces
             x_TD, weight_D = _aligned(x_TD), _aligned(weight_D)

@@ -5,10 +5,9 @@ from __future__ import annotations
 from typing import Literal
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from ._call import on_device
+from ._call import differentiable_once, on_device
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 32, 32
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -38,28 +37,28 @@ class _SelectExperts(torch.autograd.Function):
         return ids, scores
 
     @staticmethod
-    def backward(ctx, grad_ids, grad_scores):
-        if torch.is_grad_enabled():  # create_graph=True: differentiating the gradients raises
-            return _SelectExperts._backward_once(ctx, grad_ids, grad_scores)
-        return _SelectExperts._backward(ctx, grad_ids, grad_scores)
-
-    @staticmethod
-    def _backward(ctx, _, grad_scores):
+    def backward(ctx, _, grad_scores):
         if grad_scores is None:
             return None, None
         logits, ids = ctx.saved_tensors
-        top_k, sigmoid, _, _, _, _, renormalize, scale, _, _, _ = ctx.options
-        T, E = logits.shape
-        with on_device(logits.device):
-            grad_scores = grad_scores.contiguous()
-            out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-            nat.check(nat.lib.dm_select_experts_bwd(
-                logits.data_ptr(), logits.dtype is torch.bfloat16, logits.stride(0), T, E, top_k, sigmoid, renormalize, scale,
-                ids.data_ptr(), ids.dtype is torch.int64, grad_scores.data_ptr(), grad_scores.dtype is torch.bfloat16,
-                out.data_ptr(), nat.stream_ptr()), "dm_select_experts_bwd", int(T > 0))
-        return out, None
+        if not torch.is_grad_enabled():
+            return _backward(ctx.options, logits, ids, grad_scores), None
+        with torch.no_grad():
+            grad = _backward(ctx.options, logits, ids, grad_scores)
+        return *differentiable_once("select_experts", (grad,), (grad_scores, logits)), None
 
-    _backward_once = staticmethod(once_differentiable(_backward.__func__))
+
+def _backward(options, logits, ids, grad_scores):
+    top_k, sigmoid, _, _, _, _, renormalize, scale, _, _, _ = options
+    T, E = logits.shape
+    with on_device(logits.device):
+        grad_scores = grad_scores.contiguous()
+        out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+        nat.check(nat.lib.dm_select_experts_bwd(
+            logits.data_ptr(), logits.dtype is torch.bfloat16, logits.stride(0), T, E, top_k, sigmoid, renormalize, scale,
+            ids.data_ptr(), ids.dtype is torch.int64, grad_scores.data_ptr(), grad_scores.dtype is torch.bfloat16,
+            out.data_ptr(), nat.stream_ptr()), "dm_select_experts_bwd", int(T > 0))
+    return out
 
 
 def select_experts(logits_TE: torch.Tensor, top_k: int, *, score: Literal["softmax", "sigmoid"] = "softmax",
