@@ -20,10 +20,9 @@ def test_norm(residual, transposed):
     first = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)
     again = torch.autograd.grad(y.sum(), (x, w), create_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
-    for g in again:
-        for ask in (x, w):
-            with pytest.raises(RuntimeError, match="differentiate twice"):
-                torch.autograd.grad(g.float().pow(2).sum() + x.sum() + w.sum(), ask, retain_graph=True)
+    for g, ask in ((again[0], x), (again[0], w), (again[1], x)):  # the gain's gradient does not depend on the gain
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            torch.autograd.grad(g.float().pow(2).sum() + x.sum() + w.sum(), ask, retain_graph=True)
 
 
 def test_selection():
