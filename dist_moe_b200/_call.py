@@ -18,6 +18,7 @@ import os
 import sys
 
 import torch
+from torch.autograd import forward_ad
 from torch.profiler import record_function
 
 from . import _native as nat
@@ -107,6 +108,13 @@ def differentiable_once(name: str, grads: tuple, sources: tuple) -> tuple:
     that raises.  ``once_differentiable`` ties them to nothing: where the incoming gradients are constants, or where the second
     derivative is asked for by its leaves, it leaves a term out without a word."""
     return _Once.apply(name, grads, *sources)
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Forward-mode differentiation (dual tensors, ``torch.func.jvp``) ends here: a launch takes addresses, and would drop a tangent
+    without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def launch(fn, names: dict, state, k, steps: int) -> None:

@@ -11,7 +11,7 @@ import dataclasses
 import torch
 
 from . import _native as nat
-from ._call import differentiable_once, on_device
+from ._call import differentiable_once, on_device, refuse_tangents
 
 _TYPES = (torch.bfloat16, torch.float32)
 _FLOAT32 = torch.finfo(torch.float32)  # what the kernels take eps and the centre as
@@ -188,6 +188,7 @@ def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: tor
             raise ValueError("quantised rows need D to be a multiple of 32 and at most 16384")
         if grads:
             raise RuntimeError("quantised rows have no gradient: call add_rms_norm(quantize=True) under torch.no_grad()")
+    refuse_tangents("add_rms_norm", x_TD, residual_TD, weight_D)
     if not weight_D.is_contiguous():
         weight_D = weight_D.contiguous()
     if grads:

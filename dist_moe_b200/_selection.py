@@ -7,7 +7,7 @@ from typing import Literal
 import torch
 
 from . import _native as nat
-from ._call import differentiable_once, on_device
+from ._call import differentiable_once, on_device, refuse_tangents
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 32, 32
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -119,6 +119,7 @@ def select_experts(logits_TE: torch.Tensor, top_k: int, *, score: Literal["softm
             raise ValueError(f"token_mask_T must have shape [{T}]")
     if device.type != "cuda" or any(t is not None and t.device != device for t in (bias_E, token_mask_T)):
         raise ValueError("all operation tensors must reside on the same CUDA device")
+    refuse_tangents("select_experts", logits_TE, bias_E)
     if logits_TE.stride(1) != 1 and E > 1:
         logits_TE = logits_TE.contiguous()
     if bias_E is not None and not bias_E.is_contiguous():

@@ -688,7 +688,7 @@ def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tens
     if isinstance(w13_weight, PreparedWeight) or isinstance(w2_weight, PreparedWeight) or context.config.block_scaled is not None:
         raise ValueError("routed_experts_few_tokens runs on BF16 contexts with tensor weights")
     from . import _few_tokens
-    from ._call import on_device
+    from ._call import on_device, refuse_tangents
 
     state = context._state
     if state.ep != 1:
@@ -709,6 +709,7 @@ def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tens
                          "a top_k of at most 32")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x_TD, topk_scores_TK, w13_EFD, w2_EDF)):
         raise RuntimeError("routed_experts_few_tokens is forward-only: call it under torch.no_grad() or use routed_experts")
+    refuse_tangents("routed_experts_few_tokens", x_TD, topk_scores_TK, w13_EFD, w2_EDF)
     if x_TD.data_ptr() % 16:
         x_TD = x_TD.clone()
     if w13_EFD.data_ptr() % 16 or w2_EDF.data_ptr() % 16:
