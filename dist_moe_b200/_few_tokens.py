@@ -10,18 +10,27 @@ MAX_TOKENS = 64  # DM_FEW_TOKENS_MAX
 COUNTER_BYTES = 8192  # DM_FEW_TOKENS_COUNTER_BYTES
 
 
-def workspace(state) -> torch.Tensor | None:
-    """What a context keeps for calls of few tokens, None where they are not offered.  The context clears its counters."""
+def workspace_bytes(state) -> int:
+    """Not positive where calls of few tokens are not offered for the context's sizes."""
     cfg = state.config
-    if state.ep != 1 or state.block_scaled:
-        return None
-    nbytes = nat.lib.dm_few_tokens_workspace_bytes(min(MAX_TOKENS, cfg.max_num_local_input_tokens), cfg.hidden_dim,
-                                                   cfg.intermediate_dim, cfg.num_experts, cfg.top_k)
-    return torch.empty(nbytes, dtype=torch.uint8, device=state.device) if nbytes > 0 else None
+    return nat.lib.dm_few_tokens_workspace_bytes(min(MAX_TOKENS, cfg.max_num_local_input_tokens), cfg.hidden_dim, cfg.intermediate_dim,
+                                                 cfg.num_experts, cfg.top_k)
+
+
+def workspace(state) -> torch.Tensor:
+    """The context's workspace, taken by its first call; the context clears its counters from then on.  A graph that is captured before
+    has one of its own in its memory pool, cleared by every replay: an eager call may come in between."""
+    ws = state.few_workspace
+    if ws is None:
+        ws = torch.empty(workspace_bytes(state), dtype=torch.uint8, device=state.device)
+        ws[:COUNTER_BYTES].zero_()
+        if not torch.cuda.is_current_stream_capturing():
+            state.few_workspace = ws
+    return ws
 
 
 def run(x, ids, scores, w13, w2, state) -> torch.Tensor:
-    cfg, ws = state.config, state.few_workspace
+    cfg, ws = state.config, workspace(state)
     out = torch.empty_like(x)
     nat.check(nat.lib.dm_few_tokens(
         x.data_ptr(), ids.data_ptr(), ids.dtype is torch.int64, scores.data_ptr(), scores.dtype is torch.bfloat16, w13.data_ptr(),

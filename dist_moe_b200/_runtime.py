@@ -136,7 +136,7 @@ class ContextState:
             self.route_workspace_words = words
             self.gather_flags = torch.zeros(self.capacity_rows // 128 + 8 + ep_size * self.e_local * T // 128,
                                             dtype=torch.int32, device=device)
-            self.few_workspace = _few_tokens.workspace(self)
+            self.few_workspace = None  # _few_tokens.workspace
             self.reset()
         if config.block_scaled is not None:
             ob, vpe, sb, vec, gs = format_constants(config.block_scaled.format)

@@ -704,7 +704,7 @@ def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tens
         raise ValueError(f"x_TD is on {x_TD.device} but the context was created on {state.device}")
     if x_TD.shape[0] > _few_tokens.MAX_TOKENS:
         raise ValueError(f"routed_experts_few_tokens takes at most {_few_tokens.MAX_TOKENS} tokens, got {x_TD.shape[0]}")
-    if state.few_workspace is None:
+    if state.few_workspace is None and _few_tokens.workspace_bytes(state) <= 0:
         raise ValueError("routed_experts_few_tokens needs an intermediate dimension of whole multiples of 8, at most 1024 experts and "
                          "a top_k of at most 32")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x_TD, topk_scores_TK, w13_EFD, w2_EDF)):
