@@ -311,6 +311,11 @@ def _rmsnorm_args(post):
     return (None, False, 1e-6, torch.float32, torch.bfloat16, False, 0.0, False, False)
 
 
+_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_pre_dispatch_modes = torch._ops.mode_stack_state_for_pre_dispatch().count
+_functorch_level, _jit_tracing = torch._C._functorch.peek_interpreter_stack, torch._C._is_tracing
+
+
 def _plain_execution(*tensors) -> bool:
     """Nothing acts on this call's operators: no tracing or fake tensors, no dispatch or function mode, no functorch
     level, no recorder (profiler, execution trace).  The registered operators' bodies can then run without the dispatcher,
@@ -321,10 +326,7 @@ def _plain_execution(*tensors) -> bool:
         kind = type(t)
         if kind is not torch.Tensor and kind is not torch.nn.Parameter:
             return False
-    c = torch._C
-    return (not recorded() and c._len_torch_dispatch_stack() == 0 and c._len_torch_function_stack() == 0
-            and torch._ops._len_torch_dispatch_stack_pre_dispatch() == 0
-            and c._functorch.peek_interpreter_stack() is None and c._get_tracing_state() is None)
+    return not (recorded() or _modes() or _function_modes() or _pre_dispatch_modes() or _jit_tracing()) and _functorch_level() is None
 
 
 class _RegisteredBf16Function(torch.autograd.Function):

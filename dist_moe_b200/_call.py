@@ -110,6 +110,11 @@ def differentiable_once(name: str, grads: tuple, sources: tuple) -> tuple:
     return _Once.apply(name, grads, *sources)
 
 
+def has_address(t: torch.Tensor) -> bool:
+    """Not a fake tensor or another stand-in."""
+    return type(t) is torch.Tensor or type(t) is torch.nn.Parameter
+
+
 def refuse_tangents(name: str, *tensors) -> None:
     """Forward-mode differentiation (dual tensors, ``torch.func.jvp``) ends here: a launch takes addresses, and would drop a tangent
     without a word."""

@@ -5,6 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
+from ._call import on_device
 
 MAX_TOKENS = 64  # DM_FEW_TOKENS_MAX
 COUNTER_BYTES = 8192  # DM_FEW_TOKENS_COUNTER_BYTES
@@ -29,12 +30,26 @@ def workspace(state) -> torch.Tensor:
     return ws
 
 
+def checked_run(x, ids, scores, w13, w2, context) -> torch.Tensor:
+    from .api import _few_tokens_arguments
+
+    return run(*_few_tokens_arguments(x, ids, scores, w13, w2, context), context._state)
+
+
 def run(x, ids, scores, w13, w2, state) -> torch.Tensor:
-    cfg, ws = state.config, workspace(state)
-    out = torch.empty_like(x)
-    nat.check(nat.lib.dm_few_tokens(
-        x.data_ptr(), ids.data_ptr(), ids.dtype is torch.int64, scores.data_ptr(), scores.dtype is torch.bfloat16, w13.data_ptr(),
-        w2.data_ptr(), out.data_ptr(), x.shape[0], cfg.hidden_dim, cfg.intermediate_dim, cfg.num_experts, cfg.top_k,
-        cfg.activation == "swiglu_clamped", cfg.swiglu_alpha, cfg.swiglu_limit, ws.data_ptr(), ws.numel(), state.num_sms,
-        state.status.data_ptr(), nat.stream_ptr()), "dm_few_tokens")
+    if x.data_ptr() % 16:
+        x = x.clone()
+    w13_ptr, w2_ptr = w13.data_ptr(), w2.data_ptr()
+    if w13_ptr % 16 or w2_ptr % 16:
+        raise ValueError("w13_EFD and w2_EDF must start on a 16-byte boundary")
+    with on_device(state.device):
+        cfg, ws = state.config, state.few_workspace
+        if ws is None:
+            ws = workspace(state)
+        out = torch.empty_like(x)
+        nat.check(nat.lib.dm_few_tokens(
+            x.data_ptr(), ids.data_ptr(), ids.dtype is torch.int64, scores.data_ptr(), scores.dtype is torch.bfloat16, w13_ptr,
+            w2_ptr, out.data_ptr(), x.shape[0], cfg.hidden_dim, cfg.intermediate_dim, cfg.num_experts, cfg.top_k,
+            cfg.activation == "swiglu_clamped", cfg.swiglu_alpha, cfg.swiglu_limit, ws.data_ptr(), ws.numel(), state.num_sms,
+            state.status.data_ptr(), nat.stream_ptr()), "dm_few_tokens")
     return out

@@ -11,10 +11,11 @@ import dataclasses
 import torch
 
 from . import _native as nat
-from ._call import differentiable_once, on_device, refuse_tangents
+from ._bf16 import _plain_execution
+from ._call import differentiable_once, has_address, on_device, refuse_tangents
 
 _TYPES = (torch.bfloat16, torch.float32)
-_FLOAT32 = torch.finfo(torch.float32)  # what the kernels take eps and the centre as
+_TINY, _LARGEST = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max  # what the kernels take eps and the centre as
 
 
 @dataclasses.dataclass(frozen=True, eq=False)
@@ -31,7 +32,7 @@ class QuantizedRows:
             raise TypeError("packed must be a CUDA uint8 tensor")
         if isinstance(D, bool) or not isinstance(D, int) or D <= 0 or D % 32:
             raise ValueError("hidden_dim must be a positive multiple of 32")
-        if t.ndim != 2 or t.shape[1] != _row_bytes(D) or not t.is_contiguous() or t.data_ptr() % 16:
+        if t.ndim != 2 or t.shape[1] != _row_bytes(D) or not t.is_contiguous() or (has_address(t) and t.data_ptr() % 16):
             raise ValueError(f"packed must be a contiguous, 16-byte aligned tensor of shape [T, {_row_bytes(D)}]")
 
     @property
@@ -46,12 +47,18 @@ class QuantizedRows:
 
     def dequantize(self) -> torch.Tensor:
         """The rows' values as bf16 ``[T, hidden_dim]``: exact, but for values below 2 ** -133, which bf16 does not have."""
-        T, stride = self.packed.shape
-        with on_device(self.packed.device):
-            out = torch.empty(T, self.hidden_dim, dtype=torch.bfloat16, device=self.packed.device)
-            nat.check(nat.lib.dm_dequant_mxfp8_rows(self.packed.data_ptr(), stride, T, self.hidden_dim, out.data_ptr(),
-                                                    nat.stream_ptr()), "dm_dequant_mxfp8_rows", int(T > 0))
-        return out
+        if _plain_execution(self.packed):
+            return _dequantize(self.packed, self.hidden_dim)
+        return torch.ops.dist_moe.dequantize_mxfp8_rows(self.packed, self.hidden_dim)
+
+
+def _dequantize(packed, D):
+    T, stride = packed.shape
+    with on_device(packed.device):
+        out = torch.empty(T, D, dtype=torch.bfloat16, device=packed.device)
+        nat.check(nat.lib.dm_dequant_mxfp8_rows(packed.data_ptr(), stride, T, D, out.data_ptr(), nat.stream_ptr()),
+                  "dm_dequant_mxfp8_rows", int(T > 0))
+    return out
 
 
 def _row_bytes(dim: int) -> int:
@@ -63,22 +70,24 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _like(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+def _rows_and_result(t: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``_rows`` of ``t``, and a contiguous tensor for a result of its shape."""
+    if t.is_contiguous():
+        return t, torch.empty_like(t)
+    return _rows(t), torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _forward(x, residual, weight, eps, center, want_rstd, quantize):
     T, D = x.shape
     device = x.device
-    if not x.is_contiguous():
-        x = _rows(x)
-    y = _like(x)
+    if quantize:  # the quantiser's 16-byte pieces
+        x, weight = _aligned(x), _aligned(weight)
+        residual = None if residual is None else _aligned(residual)
+    x, y = _rows_and_result(x)
     total = residual_ptr = total_ptr = None
     residual_stride = residual_f32 = 0
     if residual is not None:
-        if not residual.is_contiguous():
-            residual = _rows(residual)
-        total = _like(residual)
+        residual, total = _rows_and_result(residual)
         residual_ptr, total_ptr, residual_stride = residual.data_ptr(), total.data_ptr(), residual.stride(0)
         residual_f32 = residual.dtype is torch.float32
     rstd = torch.empty(T, dtype=torch.float32, device=device) if want_rstd else None
@@ -88,18 +97,27 @@ def _forward(x, residual, weight, eps, center, want_rstd, quantize):
         rows = torch.empty((T, stride), dtype=torch.uint8, device=device)
     nat.check(nat.lib.dm_add_rmsnorm_fwd(
         x.data_ptr(), x.stride(0), residual_ptr, residual_f32, residual_stride, weight.data_ptr(), weight.dtype is torch.float32,
-        center, eps, T, D, total_ptr, y.data_ptr(), nat.ptr(rstd), nat.ptr(rows), stride, nat.stream_ptr()),
+        center, eps, T, D, total_ptr, y.data_ptr(), None if rstd is None else rstd.data_ptr(),
+        None if rows is None else rows.data_ptr(), stride, nat.stream_ptr()),
         "dm_add_rmsnorm_fwd", int(T > 0))
-    return x, y, total, rstd, rows
+    return y, total, rstd, rows
+
+
+def _forward_seen(x, residual, weight, eps, center, want_rstd, quantize):
+    """``_forward``, through the registered operator where something acts on operators."""
+    if _plain_execution(x, weight, x if residual is None else residual):
+        with on_device(x.device):
+            return _forward(x, residual, weight, eps, center, want_rstd, quantize)
+    y, total, rstd, rows = torch.ops.dist_moe.add_rms_norm(x, residual, weight, float(eps), float(center), want_rstd, quantize)
+    return y, None if residual is None else total, rstd if want_rstd else None, rows if quantize else None
 
 
 class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps, center):
-        with on_device(x.device):
-            kept, y, total, rstd, _ = _forward(x, residual, weight, eps, center, True, False)
+        y, total, rstd, _ = _forward_seen(x, residual, weight, eps, center, True, False)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(kept if residual is None else total, weight, rstd)
+        ctx.save_for_backward(x if residual is None else total, weight, rstd)
         ctx.center = center
         return y if residual is None else (y, total)
 
@@ -113,25 +131,34 @@ class _AddRmsNorm(torch.autograd.Function):
             return (grad_sum.to(torch.bfloat16) if want_x else None, grad_sum if want_residual else None,
                     torch.zeros_like(weight) if want_weight else None, None, None)
         if not torch.is_grad_enabled():
-            return *_backward(ctx, grad_y, grad_sum, total, weight, rstd), None, None
+            return *_backward_seen(ctx, grad_y, grad_sum, total, weight, rstd), None, None
         with torch.no_grad():
-            gx, gr, gw = _backward(ctx, grad_y, grad_sum, total, weight, rstd)
+            gx, gr, gw = _backward_seen(ctx, grad_y, grad_sum, total, weight, rstd)
         gx, gr = differentiable_once("add_rms_norm", (gx, gr), (grad_y, grad_sum, total, weight))
         gw, = differentiable_once("add_rms_norm", (gw,), (grad_y, total if want_x or want_residual else None))
         return gx, gr, gw, None, None
 
 
-def _backward(ctx, grad_y, grad_sum, total, weight, rstd):
+def _backward_seen(ctx, grad_y, grad_sum, total, weight, rstd):
     want_x, want_residual, want_weight = ctx.needs_input_grad[:3]
-    T, D = grad_y.shape
-    device = grad_y.device
     apart = total.dtype is torch.float32
-    with on_device(device):
+    wanted = want_x or (want_residual and not apart), want_residual and apart, want_weight
+    if _plain_execution(grad_y, total, weight):
+        gx, gr, gw = _backward(grad_y, grad_sum, total, weight, rstd, ctx.center, *wanted)
+    else:
+        grads = torch.ops.dist_moe.add_rms_norm_backward(grad_y, grad_sum, total, weight, rstd, ctx.center, *wanted)
+        gx, gr, gw = (g if want else None for g, want in zip(grads, wanted))
+    return gx if want_x else None, (gr if apart else gx) if want_residual else None, gw
+
+
+def _backward(grad_y, grad_sum, total, weight, rstd, center, want_bf16, want_float32, want_weight):
+    T, D = grad_y.shape
+    with on_device(grad_y.device):
         grad_y = grad_y.contiguous()
         if grad_sum is not None:
             grad_sum = grad_sum.contiguous()
-        gx = torch.empty_like(grad_y) if want_x or (want_residual and not apart) else None
-        gr = torch.empty_like(total) if want_residual and apart else None
+        gx = torch.empty_like(grad_y) if want_bf16 else None
+        gr = torch.empty_like(total) if want_float32 else None
         gw = partial = None
         if want_weight:
             gw = torch.empty_like(weight)
@@ -140,25 +167,13 @@ def _backward(ctx, grad_y, grad_sum, total, weight, rstd):
             gw = gw.zero_() if want_weight else None
         else:
             nat.check(nat.lib.dm_add_rmsnorm_bwd(
-                grad_y.data_ptr(), nat.ptr(grad_sum), total.data_ptr(), apart, total.stride(0), weight.data_ptr(),
-                weight.dtype is torch.float32, ctx.center, rstd.data_ptr(), T, D, nat.ptr(gx), nat.ptr(gr), nat.ptr(partial),
+                grad_y.data_ptr(), nat.ptr(grad_sum), total.data_ptr(), total.dtype is torch.float32, total.stride(0), weight.data_ptr(),
+                weight.dtype is torch.float32, center, rstd.data_ptr(), T, D, nat.ptr(gx), nat.ptr(gr), nat.ptr(partial),
                 nat.ptr(gw), nat.stream_ptr()), "dm_add_rmsnorm_bwd", 2 if want_weight else 1)
-    return gx if want_x else None, (gr if apart else gx) if want_residual else None, gw
+    return gx, gr, gw
 
 
-def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: torch.Tensor | None = None, eps: float = 1e-6,
-                 gain_center: float = 0.0, quantize: bool = False):
-    """Add ``x_TD`` to the residual stream and normalise the sum for the next layer.
-
-    ``sum = x + residual`` rounded to the residual's type (bf16 or float32; without a residual ``sum`` is ``x_TD`` itself) and
-    ``y = bf16(sum / sqrt(mean(sum ** 2) + eps) * (weight + gain_center))``: the stored sum is what is normalised.  Returns
-    ``(y_TD, sum_TD)``, differentiable in ``x_TD``, ``residual_TD`` and ``weight_D`` (bf16 or float32).  Rows may lie apart (a slice
-    of a wider tensor); other layouts are copied.
-
-    With ``quantize=True`` returns ``(y_TD, sum_TD, rows)``: ``rows`` are the MXFP8 :class:`QuantizedRows` of ``y_TD``, which
-    :func:`routed_experts` takes on MXFP8 contexts in forward-only calls, with the result that ``y_TD`` gives.  They have no
-    gradient: where one would be recorded the call raises.  ``hidden_dim`` must be a multiple of 32, at most 16384.
-    """
+def _check(x_TD, weight_D, residual_TD, eps, gain_center, quantize) -> None:
     if not isinstance(x_TD, torch.Tensor) or x_TD.dtype != torch.bfloat16:
         raise TypeError("x_TD must be a torch.bfloat16 tensor")
     if not isinstance(weight_D, torch.Tensor) or weight_D.dtype not in _TYPES:
@@ -175,19 +190,34 @@ def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: tor
     device = x_TD.device
     if device.type != "cuda" or weight_D.device != device or (residual_TD is not None and residual_TD.device != device):
         raise ValueError("all operation tensors must reside on the same CUDA device")
-    if not isinstance(eps, (int, float)) or not _FLOAT32.tiny <= eps <= _FLOAT32.max:
+    if not isinstance(eps, (int, float)) or not _TINY <= eps <= _LARGEST:
         raise ValueError("eps must be finite and positive, in float32 too")
-    if not isinstance(gain_center, (int, float)) or not abs(gain_center) <= _FLOAT32.max:
+    if not isinstance(gain_center, (int, float)) or not abs(gain_center) <= _LARGEST:
         raise ValueError("gain_center must be finite, in float32 too")
     if not isinstance(quantize, bool):
         raise TypeError("quantize must be a bool")
+    if quantize and (D % 32 or D > 16384):
+        raise ValueError("quantised rows need D to be a multiple of 32 and at most 16384")
+
+
+def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: torch.Tensor | None = None, eps: float = 1e-6,
+                 gain_center: float = 0.0, quantize: bool = False):
+    """Add ``x_TD`` to the residual stream and normalise the sum for the next layer.
+
+    ``sum = x + residual`` rounded to the residual's type (bf16 or float32; without a residual ``sum`` is ``x_TD`` itself) and
+    ``y = bf16(sum / sqrt(mean(sum ** 2) + eps) * (weight + gain_center))``: the stored sum is what is normalised.  Returns
+    ``(y_TD, sum_TD)``, differentiable in ``x_TD``, ``residual_TD`` and ``weight_D`` (bf16 or float32).  Rows may lie apart (a slice
+    of a wider tensor); other layouts are copied.
+
+    With ``quantize=True`` returns ``(y_TD, sum_TD, rows)``: ``rows`` are the MXFP8 :class:`QuantizedRows` of ``y_TD``, which
+    :func:`routed_experts` takes on MXFP8 contexts in forward-only calls, with the result that ``y_TD`` gives.  They have no
+    gradient: where one would be recorded the call raises.  ``hidden_dim`` must be a multiple of 32, at most 16384.
+    """
+    _check(x_TD, weight_D, residual_TD, eps, gain_center, quantize)
     grads = torch.is_grad_enabled() and (x_TD.requires_grad or weight_D.requires_grad
                                          or (residual_TD is not None and residual_TD.requires_grad))
-    if quantize:
-        if D % 32 or D > 16384:
-            raise ValueError("quantised rows need D to be a multiple of 32 and at most 16384")
-        if grads:
-            raise RuntimeError("quantised rows have no gradient: call add_rms_norm(quantize=True) under torch.no_grad()")
+    if quantize and grads:
+        raise RuntimeError("quantised rows have no gradient: call add_rms_norm(quantize=True) under torch.no_grad()")
     refuse_tangents("add_rms_norm", x_TD, residual_TD, weight_D)
     if not weight_D.is_contiguous():
         weight_D = weight_D.contiguous()
@@ -196,14 +226,10 @@ def add_rms_norm(x_TD: torch.Tensor, weight_D: torch.Tensor, *, residual_TD: tor
             kept = _rows(x_TD)  # what is saved is what the gradients depend on
             return _AddRmsNorm.apply(kept, None, weight_D, float(eps), float(gain_center)), x_TD
         return _AddRmsNorm.apply(x_TD, residual_TD, weight_D, float(eps), float(gain_center))
-    with on_device(device):
-        if quantize:  # the quantiser's 16-byte pieces
-            x_TD, weight_D = _aligned(x_TD), _aligned(weight_D)
-            residual_TD = None if residual_TD is None else _aligned(residual_TD)
-        _, y, total, _, rows = _forward(x_TD, residual_TD, weight_D, eps, gain_center, False, quantize)
+    y, total, _, rows = _forward_seen(x_TD, residual_TD, weight_D, eps, gain_center, False, quantize)
     if residual_TD is None:
         total = x_TD
-    return (y, total, QuantizedRows(rows, D)) if quantize else (y, total)
+    return (y, total, QuantizedRows(rows, int(x_TD.shape[1]))) if quantize else (y, total)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

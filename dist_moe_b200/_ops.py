@@ -13,6 +13,10 @@ rows per local expert ``int32[E_local]``, backward gather pointers, forward gath
 (``int64[P]`` each), rows per rank ``int32[EP]``, rows received ``int32[1]``, recompute flag ``uint8[1]``,
 planner state ``int64[6]``, rstd ``fp32[T, K]`` (empty without RMSNorm).
 
+Besides the reference's ten there are this library's own for what stands around the experts (``AROUND``): ``add_rms_norm``,
+``add_rms_norm_backward``, ``dequantize_mxfp8_rows``, ``select_experts``, ``select_experts_backward`` and
+``routed_experts_few_tokens``.  Outputs that were not asked for come back empty.
+
 Importing this module registers the operators once per process; if another library already defined an
 operator of the same name (the reference imported next to this package) that definition is left alone.
 """
@@ -26,6 +30,7 @@ from .formats import BlockScaledFormat
 
 _NS = "dist_moe"
 REGISTERED: list[str] = []
+AROUND: list[str] = []
 
 
 def _context(context_id: str):
@@ -479,8 +484,128 @@ def _register_block_scaled() -> None:
                        "block_scaled_backward_accumulate_"])
 
 
+# ---------------------------------------------------------------------------------------------
+# Around the experts
+# ---------------------------------------------------------------------------------------------
+def _register_around_the_experts() -> None:
+    def empty(t, shape=(0,), dtype=None):
+        return torch.empty(shape, dtype=dtype or t.dtype, device=t.device)
+
+    def expect(ok: bool, what: str) -> None:
+        if not ok:
+            raise RuntimeError(what)
+
+    @torch.library.custom_op(f"{_NS}::add_rms_norm", mutates_args=(), device_types="cuda")
+    def add_rms_norm(x_TD: torch.Tensor, residual_TD: torch.Tensor | None, weight_D: torch.Tensor, eps: float, gain_center: float,
+                     want_rstd: bool, quantize: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        from . import _norm
+        from ._call import on_device
+
+        _norm._check(x_TD, weight_D, residual_TD, eps, gain_center, quantize)
+        with on_device(x_TD.device):
+            y, total, rstd, rows = _norm._forward(x_TD, residual_TD, weight_D.contiguous(), eps, gain_center, want_rstd, quantize)
+        return (y, empty(x_TD) if total is None else total, empty(x_TD, dtype=torch.float32) if rstd is None else rstd,
+                empty(x_TD, dtype=torch.uint8) if rows is None else rows)
+
+    @add_rms_norm.register_fake
+    def _(x_TD, residual_TD, weight_D, eps, gain_center, want_rstd, quantize):
+        from ._norm import _row_bytes
+
+        T, D = x_TD.shape
+        return (empty(x_TD, (T, D)), empty(x_TD) if residual_TD is None else empty(residual_TD, (T, D)),
+                empty(x_TD, (T,) if want_rstd else (0,), torch.float32), empty(x_TD, (T, _row_bytes(D)) if quantize else (0,), torch.uint8))
+
+    @torch.library.custom_op(f"{_NS}::add_rms_norm_backward", mutates_args=(), device_types="cuda")
+    def add_rms_norm_backward(grad_y_TD: torch.Tensor, grad_sum_TD: torch.Tensor | None, sum_TD: torch.Tensor, weight_D: torch.Tensor,
+                              rstd_T: torch.Tensor, gain_center: float, want_bf16: bool, want_float32: bool,
+                              want_weight: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        from . import _norm
+
+        expect(sum_TD.ndim == 2 and sum_TD.dtype in _norm._TYPES and grad_y_TD.shape == sum_TD.shape and grad_y_TD.dtype == torch.bfloat16
+               and (grad_sum_TD is None or (grad_sum_TD.shape == sum_TD.shape and grad_sum_TD.dtype == sum_TD.dtype)),
+               "gradients of the norm do not match the sum")
+        expect(weight_D.shape == sum_TD.shape[1:] and weight_D.dtype in _norm._TYPES and rstd_T.shape == sum_TD.shape[:1]
+               and rstd_T.dtype == torch.float32 and (not want_float32 or sum_TD.dtype == torch.float32),
+               "what the norm's forward kept does not match the sum")
+        expect(all(t is None or t.device == grad_y_TD.device for t in (grad_sum_TD, sum_TD, weight_D, rstd_T)),
+               "all operation tensors must reside on the same CUDA device")
+        grads = _norm._backward(grad_y_TD, grad_sum_TD, _norm._rows(sum_TD), weight_D.contiguous(), rstd_T.contiguous(), gain_center,
+                                want_bf16, want_float32, want_weight)
+        return tuple(empty(t) if g is None else g for g, t in zip(grads, (grad_y_TD, sum_TD, weight_D)))
+
+    @add_rms_norm_backward.register_fake
+    def _(grad_y_TD, grad_sum_TD, sum_TD, weight_D, rstd_T, gain_center, want_bf16, want_float32, want_weight):
+        return (empty(grad_y_TD, grad_y_TD.shape if want_bf16 else (0,)), empty(sum_TD, sum_TD.shape if want_float32 else (0,)),
+                empty(weight_D, weight_D.shape if want_weight else (0,)))
+
+    @torch.library.custom_op(f"{_NS}::dequantize_mxfp8_rows", mutates_args=(), device_types="cuda")
+    def dequantize_mxfp8_rows(packed: torch.Tensor, hidden_dim: int) -> torch.Tensor:
+        from . import _norm
+
+        _norm.QuantizedRows(packed, hidden_dim)  # its checks
+        return _norm._dequantize(packed, hidden_dim)
+
+    @dequantize_mxfp8_rows.register_fake
+    def _(packed, hidden_dim):
+        return empty(packed, (packed.shape[0], hidden_dim), torch.bfloat16)
+
+    @torch.library.custom_op(f"{_NS}::select_experts", mutates_args=(), device_types="cuda")
+    def select_experts(logits_TE: torch.Tensor, bias_E: torch.Tensor | None, token_mask_T: torch.Tensor | None, top_k: int, score: str,
+                       num_groups: int, num_kept_groups: int, group_top: int, renormalize: bool, scale: float, ids_dtype: torch.dtype,
+                       scores_dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+        from . import _selection
+        from ._call import on_device
+
+        _selection._check(logits_TE, top_k, score, bias_E, num_groups, num_kept_groups, group_top, renormalize, scale, token_mask_T,
+                          ids_dtype, scores_dtype)
+        logits, bias, mask = _selection._laid_out(logits_TE, bias_E, token_mask_T)
+        with on_device(logits.device):
+            return _selection._forward(logits, (top_k, score == "sigmoid", bias, num_groups, num_kept_groups, group_top, renormalize,
+                                                scale, mask, ids_dtype, scores_dtype))
+
+    @select_experts.register_fake
+    def _(logits_TE, bias_E, token_mask_T, top_k, score, num_groups, num_kept_groups, group_top, renormalize, scale, ids_dtype,
+          scores_dtype):
+        shape = logits_TE.shape[0], top_k
+        return empty(logits_TE, shape, ids_dtype), empty(logits_TE, shape, scores_dtype)
+
+    @torch.library.custom_op(f"{_NS}::select_experts_backward", mutates_args=(), device_types="cuda")
+    def select_experts_backward(logits_TE: torch.Tensor, topk_expert_ids_TK: torch.Tensor, grad_scores_TK: torch.Tensor, score: str,
+                                renormalize: bool, scale: float) -> torch.Tensor:
+        from . import _selection
+
+        expect(logits_TE.ndim == topk_expert_ids_TK.ndim == 2 and logits_TE.dtype in _selection._FLOATS
+               and topk_expert_ids_TK.shape[0] == logits_TE.shape[0] and topk_expert_ids_TK.shape == grad_scores_TK.shape
+               and topk_expert_ids_TK.dtype in (torch.int32, torch.int64) and grad_scores_TK.dtype in _selection._FLOATS
+               and score in ("softmax", "sigmoid"), "gradients of the selection do not match the logits")
+        expect(logits_TE.device == topk_expert_ids_TK.device == grad_scores_TK.device,
+               "all operation tensors must reside on the same CUDA device")
+        logits, _, _ = _selection._laid_out(logits_TE, None, None)
+        return _selection._backward(logits, topk_expert_ids_TK.contiguous(), grad_scores_TK, score == "sigmoid", renormalize, scale)
+
+    @select_experts_backward.register_fake
+    def _(logits_TE, topk_expert_ids_TK, grad_scores_TK, score, renormalize, scale):
+        return empty(logits_TE, logits_TE.shape)
+
+    @torch.library.custom_op(f"{_NS}::routed_experts_few_tokens", mutates_args=(), device_types="cuda")
+    def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tensor, topk_scores_TK: torch.Tensor,
+                                  w13_EFD: torch.Tensor, w2_EDF: torch.Tensor, context_id: str) -> torch.Tensor:
+        from . import _few_tokens
+
+        return _few_tokens.checked_run(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, _context(context_id))
+
+    @routed_experts_few_tokens.register_fake
+    def _(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, context_id):
+        return empty(x_TD, x_TD.shape)
+
+    AROUND.extend(["add_rms_norm", "add_rms_norm_backward", "dequantize_mxfp8_rows", "select_experts", "select_experts_backward",
+                   "routed_experts_few_tokens"])
+
+
 def register() -> list[str]:
-    """Define the operators (idempotent).  Returns the names this package registered."""
+    """Define the operators (idempotent).  Returns the names of the reference's operators that this package registered."""
+    if not AROUND:
+        _register_around_the_experts()
     if REGISTERED:
         return list(REGISTERED)
     existing = getattr(torch.ops, _NS)

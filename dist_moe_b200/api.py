@@ -19,7 +19,9 @@ from typing import Any, Literal, get_args
 import torch
 import torch.distributed as dist
 
-from . import _planning
+from . import _few_tokens, _planning
+from ._bf16 import _plain_execution
+from ._call import refuse_tangents
 from ._execution import DEFAULT_OPTIONS, ExecutionOptions, PreparedWeight, RMSNormPostprocess
 from ._norm import QuantizedRows
 from .formats import (
@@ -681,15 +683,21 @@ def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tens
     from ``routed_experts`` in rounding.  On large layers ``routed_experts`` is faster beyond some five tokens per expert hit.  Calls on
     one context are ordered, graph replays included: they share its workspace.
     """
+    x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF = _few_tokens_arguments(x_TD, topk_expert_ids_TK, topk_scores_TK,
+                                                                                  w13_weight, w2_weight, context)
+    if _plain_execution(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF):
+        return _few_tokens.run(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, context._state)
+    return torch.ops.dist_moe.routed_experts_few_tokens(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, context._context_id)
+
+
+def _few_tokens_arguments(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_weight, w2_weight, context: Context):
+    """The checked arguments of a call of few tokens."""
     if not isinstance(context, Context):
         raise TypeError("context must come from create_context()")
     if context._closed:
         raise RuntimeError("distributed MoE context is closed")
     if isinstance(w13_weight, PreparedWeight) or isinstance(w2_weight, PreparedWeight) or context.config.block_scaled is not None:
         raise ValueError("routed_experts_few_tokens runs on BF16 contexts with tensor weights")
-    from . import _few_tokens
-    from ._call import on_device, refuse_tangents
-
     state = context._state
     if state.ep != 1:
         raise ValueError("routed_experts_few_tokens needs all experts on one rank")
@@ -710,12 +718,7 @@ def routed_experts_few_tokens(x_TD: torch.Tensor, topk_expert_ids_TK: torch.Tens
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x_TD, topk_scores_TK, w13_EFD, w2_EDF)):
         raise RuntimeError("routed_experts_few_tokens is forward-only: call it under torch.no_grad() or use routed_experts")
     refuse_tangents("routed_experts_few_tokens", x_TD, topk_scores_TK, w13_EFD, w2_EDF)
-    if x_TD.data_ptr() % 16:
-        x_TD = x_TD.clone()
-    if w13_EFD.data_ptr() % 16 or w2_EDF.data_ptr() % 16:
-        raise ValueError("w13_EFD and w2_EDF must start on a 16-byte boundary")
-    with on_device(state.device):
-        return _few_tokens.run(x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF, state)
+    return x_TD, topk_expert_ids_TK, topk_scores_TK, w13_EFD, w2_EDF
 
 
 def prepare_block_scaled_weight(weight: torch.Tensor, config: Config, *, fuse_swiglu: bool = False,
