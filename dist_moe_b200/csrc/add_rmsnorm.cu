@@ -185,9 +185,9 @@ template <typename R, int kVec>
 struct NormBwd {
   static constexpr int kWide = sizeof(R) / 2;  // 16-byte pieces of eight values of the stream
   static constexpr int kPieces = kVec * (1 + 2 * kWide);
-  static int stage_bytes(int threads) { return threads * kPieces * 16; }
+  static constexpr int stage_bytes(int threads) { return threads * kPieces * 16; }
   // Blocks of an SM: up to four.
-  static int resident(int threads, int stages) {
+  static constexpr int resident(int threads, int stages) {
     const int fit = 220 * 1024 / (stages * stage_bytes(threads) + 2048), most = kNormThreads * 2 / threads;
     return fit < 4 ? (fit < most ? fit : most) : (4 < most ? 4 : most);
   }
@@ -480,11 +480,13 @@ static int add_rmsnorm_bwd(const void* grad_y, const void* grad_sum, const void*
     return static_cast<int>(cudaGetLastError());
   };
   using std::integral_constant;
-  // Two stages (three were not faster), or one where they do not fit: rows of more than 8192 values with an fp32 stream.
+  // Two stages (three were not faster), or one where they do not fit: rows of more than 10240 values with an fp32 stream.
   auto run = [&](auto warp_tag, auto vec_tag, int threads) {
     using C = NormBwd<R, decltype(vec_tag)::value>;
-    if (C::resident(threads, 2) >= 1) return launch(warp_tag, vec_tag, integral_constant<int, 2>{}, threads);
-    return launch(warp_tag, vec_tag, integral_constant<int, 1>{}, threads);
+    constexpr bool always_fit = C::resident(decltype(warp_tag)::value ? 128 : kNormThreads, 2) >= 1;
+    if constexpr (!always_fit)
+      if (C::resident(threads, 2) < 1) return launch(warp_tag, vec_tag, integral_constant<int, 1>{}, threads);
+    return launch(warp_tag, vec_tag, integral_constant<int, 2>{}, threads);
   };
   if (D <= 1024) return run(std::true_type{}, integral_constant<int, 4>{}, 128);
   if (vec <= 2 * kNormThreads) return run(std::false_type{}, integral_constant<int, 2>{}, norm_threads(vec, 2));
