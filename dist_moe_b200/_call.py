@@ -115,6 +115,15 @@ def has_address(t: torch.Tensor) -> bool:
     return type(t) is torch.Tensor or type(t) is torch.nn.Parameter
 
 
+def traced() -> bool:
+    """Operators are being written down: by ``make_fx`` or by ``torch.jit.trace``."""
+    if torch.compiler.is_compiling():  # such a tracer of Python code goes around what it does not know
+        return False
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+    return torch._C._is_tracing() or get_proxy_mode() is not None
+
+
 def refuse_tangents(name: str, *tensors) -> None:
     """Forward-mode differentiation (dual tensors, ``torch.func.jvp``) ends here: a launch takes addresses, and would drop a tangent
     without a word."""

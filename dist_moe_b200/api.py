@@ -21,7 +21,7 @@ import torch.distributed as dist
 
 from . import _few_tokens, _planning
 from ._bf16 import _plain_execution
-from ._call import refuse_tangents
+from ._call import refuse_tangents, traced
 from ._execution import DEFAULT_OPTIONS, ExecutionOptions, PreparedWeight, RMSNormPostprocess
 from ._norm import QuantizedRows
 from .formats import (
@@ -656,6 +656,8 @@ def routed_experts(x_TD: torch.Tensor | QuantizedRows, topk_expert_ids_TK: torch
             raise ValueError("quantised tokens require an MXFP8 context")
         if save_for_backward or options.requires_eager:
             raise RuntimeError("quantised tokens are for forward-only calls without callbacks")
+        if not _plain_execution(tokens) and traced():  # no operator takes them: a trace would hold an empty result
+            raise RuntimeError("calls with quantised tokens cannot be traced")
     from ._call import on_device
 
     # every launch below goes to the context's device and to that device's current stream

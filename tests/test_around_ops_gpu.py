@@ -151,3 +151,43 @@ def test_operators_refuse_what_the_calls_refuse():
         op.select_experts_backward(logits, ids, logits, "softmax", False, 1.0)
     with pytest.raises(RuntimeError, match="not live"):
         op.routed_experts_few_tokens(x, ids, logits[:, :K].contiguous(), x, x, "no-such-context")
+
+
+def test_quantised_tokens_are_not_traced():
+    ctx = dm.create_context(group=None, device=DEV, config=dm.Config(
+        max_num_local_input_tokens=T, hidden_dim=D, intermediate_dim=F, top_k=K, num_experts=E, max_moe_layers_per_activation_slot=1,
+        inference=True, block_scaled=dm.BlockScaledConfig()))
+    w13, w2 = (torch.randn(*s, device=DEV).bfloat16() * 0.06 for s in ((E, 2 * F, D), (E, D, F)))
+    ids, scores = torch.arange(K, device=DEV, dtype=torch.int32).expand(T, K).contiguous(), torch.rand(T, K, device=DEV)
+    x, _, w, _ = _inputs(0, None)
+
+    def call(x):
+        with torch.no_grad():
+            return dm.routed_experts(dm.add_rms_norm(x, w, quantize=True)[2], ids, scores, w13, w2, ctx)
+
+    want = call(x)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(call)(x)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, (x,), check_trace=False)
+    with _Watch(), profile(activities=[ProfilerActivity.CPU]):  # others do no harm
+        assert torch.equal(call(x), want)
+    ctx.check_status()
+    ctx.close()
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_under_a_tracer_of_python_code(serving, backend):
+    import torch._dynamo
+
+    torch._dynamo.reset()
+    inputs, compiled = _inputs(3, torch.float32), torch.compile(serving, backend=backend)
+    _equal(compiled(*inputs), serving(*inputs))
+    inputs = [t.requires_grad_() for t in inputs]
+
+    def layer(x, r, w, gate):
+        y, total = dm.add_rms_norm(x, w, residual_TD=r)
+        return y.float() * dm.select_experts(y.float() @ gate.t(), K)[1].sum(1, keepdim=True) + total
+
+    _equal(*(torch.autograd.grad(f(*inputs).sum(), inputs) for f in (torch.compile(layer, backend=backend), layer)))
+    torch._dynamo.reset()

@@ -8,6 +8,7 @@ from torch.overrides import TorchFunctionMode
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from dist_moe_b200._bf16 import _plain_execution
+from dist_moe_b200._call import traced
 
 
 def _seen(run):
@@ -47,3 +48,13 @@ def test_noticed(run):
                                  _under(lambda: torch.autocast("cpu", dtype=torch.bfloat16))])
 def test_left_alone(run):
     assert not _seen(run)
+
+
+def test_tracers_are_told_from_other_modes():
+    found = {}
+    make_fx(lambda a: found.update(make_fx=traced()) or a * 2)(torch.ones(3))
+    torch.jit.trace(lambda a: found.update(jit=traced()) or a * 2, (torch.ones(3),), check_trace=False)
+    with _Operators(), _Functions():
+        found["modes"] = traced()
+    found["nothing"] = traced()
+    assert found == {"make_fx": True, "jit": True, "modes": False, "nothing": False}
