@@ -7,15 +7,20 @@
 // Quantised rows are those of the MXFP8 row quantiser applied to y, bit for bit, in the packed form that inference calls publish:
 // D bytes E4M3, D / 32 scale bytes, padding to 16 bytes.
 //
-// HBM bound: every value of a row stays in registers between its sum and its use, 2 + 2|4 bytes in and 2 + 2|4 (+ 1.03) out per
-// element, in the backward 2 + 2|4 + 2|4 in and 2 (+ 4) out.  A row belongs to a block of as many warps as it takes with two 16-byte
-// pieces a lane (four beyond 8192 values); in the backward one of up to 1024 values to a warp, four pieces a lane, four rows to a block:
-// 16384 rows of 256 and 1024 values took 28 and 47 us so, 36 and 50 with blocks (in the forward 15 and 32 with warps, 15 and 30 with
-// blocks).  The gain's gradient is summed over the rows of a block in registers and over the blocks by a second launch, always in the
-// same order.
+// HBM bound.  Rows of whole 16-byte pieces, up to 16384 values: every value stays in registers between its sum and its use, 2 + 2|4
+// bytes in and 2 + 2|4 (+ 1.03) out per element, in the backward 2 + 2|4 + 2|4 in and 2 (+ 4) out.  A row belongs to a block of as many
+// warps as it takes with two 16-byte pieces a lane (four beyond 8192 values); in the backward one of up to 1024 values to a warp, four
+// pieces a lane, four rows to a block: 16384 rows of 256 and 1024 values took 28 and 47 us so, 36 and 50 with blocks (in the forward 15
+// and 32 with warps, 15 and 30 with blocks).  The gain's gradient is summed over the rows of a block in registers and over the blocks
+// by a second launch, always in the same order.
+// All other rows go through forms of their own (add_rmsnorm_*_any_kernel): a value a load, rows read twice, and in the backward the
+// gain's gradient of a block in memory, read and written for every row.  They take 1.4 to 2.4 times as long.
 //
-// Measured, L2 flushed, events included (some 6 us): 16384 x 4096 bf16 forward 96 us (5.6 TB/s), backward 116 us with the gain's gradient,
-// 107 without; 4096 x 2816 with an fp32 stream 29 us, with quantised rows 31 us, backward 58 us; 16 x 2048 8 us.
+// Measured, L2 flushed, events included (some 6 us): 16384 x 4096 bf16 forward 94 us (5.7 TB/s), backward 116 us with the gain's gradient,
+// 109 without; 4096 x 2816 with an fp32 stream 29 us, with quantised rows 31 us, backward 58 us (3.2 TB/s); 16384 x 1008 with a bf16 stream
+// 31 and 48, fp32 37 and 79 (3.4 TB/s), and 16384 x 1001, the other form, 59 and 116, 55 and 144; 16 x 2048 8 us.
+// What holds the backward at half of the copy rate where the stream is fp32 or a row a warp's: eight warps an SM in the warps' form, and
+// the gain, which is the same for every row that a block walks over, loaded twice a row by every thread.
 #include <type_traits>
 
 #include "quant_common.cuh"

@@ -21,7 +21,9 @@
 // lanes' largest remaining values; a lane keeps its two largest, and looks through its registers again where a third is asked for.
 //
 // Instruction bound: the logits are read once (4096 x 256 in 0.6 us at the copy rate).  Measured, events included (some 6 us), K = 8:
-// 4096 x 256 12 us from the logits alone, 14 with a bias, 17 with 4 of 8 groups too, 16384 x 256 27 and 47; backward 8 to 10 and 18.
+// 4096 x 256 12 us from the logits alone, 14 with a bias, 18 with 4 of 8 groups too, 16384 x 256 27 and 46; backward 8 to 10 and 18.
+// The backward is bound by instructions too, at one element a load and store: the softmax walks over a row three times and takes each
+// exponential twice (65536 x 256 52 us, 20 at the copy rate), the other forms fill with zeros and write K values (25 us, 10).
 #include <type_traits>
 
 #include "common.cuh"
@@ -91,7 +93,7 @@ __device__ __forceinline__ V below(float l, float top) {
   return l == top ? V(0) : V(l) - V(top);
 }
 
-// Two largest of two pairs (falling); keys, 0 = nothing.
+// The two largest values seen, falling.
 template <typename V>
 struct Top2 {
   V first, second;  // -inf: nothing
