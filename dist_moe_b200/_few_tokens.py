@@ -23,8 +23,9 @@ def workspace(state) -> torch.Tensor:
     has one of its own in its memory pool, cleared by every replay: an eager call may come in between."""
     ws = state.few_workspace
     if ws is None:
-        ws = torch.empty(workspace_bytes(state), dtype=torch.uint8, device=state.device)
-        ws[:COUNTER_BYTES].zero_()
+        with torch.inference_mode(False):  # the context clears it outside of that mode too
+            ws = torch.empty(workspace_bytes(state), dtype=torch.uint8, device=state.device)
+            ws[:COUNTER_BYTES].zero_()
         if not torch.cuda.is_current_stream_capturing():
             state.few_workspace = ws
     return ws

@@ -39,3 +39,14 @@ def test_counters_are_cleared_where_there_are_some():
 
 def test_sizes_that_are_not_offered():
     assert _few_tokens.workspace_bytes(_state(intermediate_dim=60)) < 0 and _few_tokens.workspace_bytes(_state(num_experts=1025)) < 0
+
+
+def test_a_first_call_in_inference_mode_leaves_counters_that_can_be_cleared_outside_it(monkeypatch):
+    """An inference tensor may not be written outside of that mode, and the context clears its counters there."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    state = _state()
+    with torch.inference_mode():
+        _few_tokens.workspace(state)
+    state.few_workspace.fill_(1)
+    _runtime.ContextState.clear_gather_flags(state)
+    assert not state.few_workspace[:_few_tokens.COUNTER_BYTES].any()

@@ -61,3 +61,19 @@ def test_graphs_captured_before_the_first_call():
             ctx.reset()
     ctx.check_status()
     ctx.close()
+
+
+def test_a_first_call_in_inference_mode():
+    case = _case(T, D, F, E, K)
+    ctx = _context(T, D, F, E, K)
+    with torch.inference_mode():
+        first = dm.routed_experts_few_tokens(*case, ctx)
+    ctx.reset()
+    case[1][0, 0] = E
+    dm.routed_experts_few_tokens(*case, ctx)
+    with pytest.raises(RuntimeError, match="expert id"):
+        ctx.check_status()  # clears the counters as well
+    case[1][0, 0] = _case(T, D, F, E, K)[1][0, 0]
+    assert torch.equal(dm.routed_experts_few_tokens(*case, ctx), first)
+    ctx.check_status()
+    ctx.close()
