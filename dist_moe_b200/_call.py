@@ -110,9 +110,12 @@ def differentiable_once(name: str, grads: tuple, sources: tuple) -> tuple:
     return _Once.apply(name, grads, *sources)
 
 
-def has_address(t: torch.Tensor) -> bool:
-    """Not a fake tensor or another stand-in."""
-    return type(t) is torch.Tensor or type(t) is torch.nn.Parameter
+def address(t: torch.Tensor) -> int:
+    """Where ``t`` begins; 0 for fake tensors and other stand-ins, which lie nowhere."""
+    try:
+        return t.data_ptr()
+    except RuntimeError:
+        return 0
 
 
 def traced() -> bool:

@@ -12,7 +12,7 @@ import torch
 
 from . import _native as nat
 from ._bf16 import _plain_execution
-from ._call import differentiable_once, has_address, on_device, refuse_tangents
+from ._call import address, differentiable_once, on_device, refuse_tangents
 
 _TYPES = (torch.bfloat16, torch.float32)
 _TINY, _LARGEST = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max  # what the kernels take eps and the centre as
@@ -32,7 +32,7 @@ class QuantizedRows:
             raise TypeError("packed must be a CUDA uint8 tensor")
         if isinstance(D, bool) or not isinstance(D, int) or D <= 0 or D % 32:
             raise ValueError("hidden_dim must be a positive multiple of 32")
-        if t.ndim != 2 or t.shape[1] != _row_bytes(D) or not t.is_contiguous() or (has_address(t) and t.data_ptr() % 16):
+        if t.ndim != 2 or t.shape[1] != _row_bytes(D) or not t.is_contiguous() or address(t) % 16:
             raise ValueError(f"packed must be a contiguous, 16-byte aligned tensor of shape [T, {_row_bytes(D)}]")
 
     @property

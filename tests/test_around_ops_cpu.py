@@ -100,3 +100,17 @@ def test_few_tokens(context):
             dm.routed_experts_few_tokens(*args[:4], args[4][:, :32], context)
     graph = make_fx(lambda *a: dm.routed_experts_few_tokens(*a, context), tracing_mode="fake")(*args)
     assert "dist_moe::routed_experts_few_tokens" in _nodes(graph)
+
+
+class _OnDevice(torch.Tensor):
+    """A CPU tensor that says it lies on a GPU."""
+
+    device = torch.device("cuda", 0)
+
+
+def test_rows_of_a_tensor_class_of_its_own_have_to_be_aligned_too():
+    raw = torch.zeros(2 * 48 + 16, dtype=torch.uint8)
+    first = -raw.data_ptr() % 16
+    dm.QuantizedRows(raw[first:first + 96].view(2, 48).as_subclass(_OnDevice), 32)
+    with pytest.raises(ValueError, match="aligned"):
+        dm.QuantizedRows(raw[first + 8:first + 104].view(2, 48).as_subclass(_OnDevice), 32)
