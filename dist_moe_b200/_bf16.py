@@ -19,6 +19,8 @@ from __future__ import annotations
 from typing import Any
 
 import torch
+from torch.overrides import _get_current_function_mode_stack
+from torch.utils._device import DeviceContext
 
 from . import _native as nat
 from ._call import (BWD, FWD, FWD_ALL, CallState, Layout, arguments, in_one_piece, launch, layout_of, observed, on_device,
@@ -326,7 +328,13 @@ def _plain_execution(*tensors) -> bool:
         kind = type(t)
         if kind is not torch.Tensor and kind is not torch.nn.Parameter:
             return False
-    return not (recorded() or _modes() or _function_modes() or _pre_dispatch_modes() or _jit_tracing()) and _functorch_level() is None
+    return (not (recorded() or _modes() or _pre_dispatch_modes() or _jit_tracing()) and _functorch_level() is None
+            and (not _function_modes() or _default_devices_alone()))
+
+
+def _default_devices_alone() -> bool:
+    """No function mode but a default device (``torch.set_default_device``), which means nothing to calls whose tensors are there."""
+    return all(type(mode) is DeviceContext for mode in _get_current_function_mode_stack())
 
 
 class _RegisteredBf16Function(torch.autograd.Function):

@@ -45,9 +45,22 @@ def test_noticed(run):
 
 
 @pytest.mark.parametrize("run", [_under(torch.no_grad), _under(torch.inference_mode), lambda f, x: f(torch.nn.Parameter(x)),
+                                 _under(lambda: torch.device("cpu")),
                                  _under(lambda: torch.autocast("cpu", dtype=torch.bfloat16))])
 def test_left_alone(run):
     assert not _seen(run)
+
+
+def test_a_default_device_does_not_hide_another_mode():
+    with torch.device("cpu"), _Functions():
+        assert not _plain_execution(torch.ones(3))
+    with _Functions(), torch.device("cpu"):
+        assert not _plain_execution(torch.ones(3))
+    torch.set_default_device("cpu")
+    try:
+        assert _plain_execution(torch.ones(3))
+    finally:
+        torch.set_default_device(None)
 
 
 def test_tracers_are_told_from_other_modes():
