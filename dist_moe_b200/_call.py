@@ -18,6 +18,7 @@ import os
 import sys
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
 from torch.autograd import forward_ad
 from torch.profiler import record_function
 
@@ -112,6 +113,8 @@ def differentiable_once(name: str, grads: tuple, sources: tuple) -> tuple:
 
 def address(t: torch.Tensor) -> int:
     """Where ``t`` begins; 0 for fake tensors and other stand-ins, which lie nowhere."""
+    if isinstance(t, FakeTensor):
+        return 0
     try:
         return t.data_ptr()
     except RuntimeError:
