@@ -153,6 +153,24 @@ def test_operators_refuse_what_the_calls_refuse():
         op.routed_experts_few_tokens(x, ids, logits[:, :K].contiguous(), x, x, "no-such-context")
 
 
+@pytest.mark.parametrize("mode", [torch.inference_mode, lambda: torch.device("cuda"), lambda: torch.autocast("cuda", dtype=torch.bfloat16)])
+def test_under_modes_that_change_nothing(serving, mode):
+    inputs = _inputs(3, torch.float32)
+    want = serving(*inputs)
+    for watched in (False, True):
+        watch = _Watch()
+        with mode():
+            if watched:
+                with watch:
+                    got = serving(*inputs)
+                assert sorted(watch.seen) == sorted(SERVING)
+            else:
+                got = serving(*inputs)
+        if mode is torch.inference_mode:
+            assert got[0].is_inference()
+        _equal(got[:3], want[:3])  # autocast takes the router's product in bf16
+
+
 def test_quantised_tokens_are_not_traced():
     ctx = dm.create_context(group=None, device=DEV, config=dm.Config(
         max_num_local_input_tokens=T, hidden_dim=D, intermediate_dim=F, top_k=K, num_experts=E, max_moe_layers_per_activation_slot=1,
